@@ -2,9 +2,10 @@
 ** AdamW over a list of tensors (include/anni_mtstep.h): one cooperative launch per step.
 **
 ** The list is cut into tiles of ANNI_MT_TILE elements that do not cross tensors; a table says which
-** tensor a tile belongs to.  A block takes a tile at a time, each of its eight warps one run of
+** tensor a tile belongs to.  A block takes a tile at a time, each of its eight warps runs of
 ** ANNI_MT_BLOCK = 256 elements -- the run that shares a scale in the 8-bit form, so that the two
-** block maxima are reductions inside a warp.
+** block maxima are reductions inside a warp.  The step is bound by HBM: 28 bytes per element with 32-bit
+** moments, bf16 gradients and twins, 16 with 8-bit moments.
 */
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
@@ -19,7 +20,8 @@
 #include "optstep_internal.h"
 #include "optstep_device.h"
 
-#define ANNI_MT_TILE		(ANNI_THREADS / 32 * ANNI_MT_BLOCK)
+#define ANNI_MT_PASS		(ANNI_THREADS / 32 * ANNI_MT_BLOCK)	/* elements a block takes at once */
+#define ANNI_MT_TILE		(2 * ANNI_MT_PASS)
 #define ANNI_MT_ADDRS		448	/* gradient addresses per launch of set_grads_kernel */
 
 namespace {
@@ -35,7 +37,8 @@ struct mt_desc {
 	int64_t		n;
 	uint64_t	block0;		/* blocks of 256 in the tensors before this one */
 	uint32_t	tile0;		/* tiles in the tensors before this one */
-	uint32_t	wd;
+	uint16_t	wd;
+	uint16_t	vec;		/* everything but the gradient on the alignment of the vector accesses */
 };
 
 struct mt_launch {
@@ -88,14 +91,17 @@ struct q8_hyper {
 	float	coef;
 };
 
-/* moments in float (their stored form has three and two bits of mantissa), then the shared parameter update */
+/*
+** Moments in float (their stored form has three and two bits of mantissa), every product and sum rounded on its
+** own, so that a float restatement of the formula lands on the same codes; then the shared parameter update.
+*/
 __device__ __forceinline__ void adam_q8(const anni_launch &a, const q8_hyper &h, float lrwd, float gf, float &p,
 	float &m, float &v)
 {
-	const float g = gf * h.coef;
+	const float g = __fmul_rn(gf, h.coef);
 
-	m = fmaf(h.b1, m, h.omb1 * g);
-	v = fmaf(h.b2, v, h.omb2 * g * g);
+	m = __fadd_rn(__fmul_rn(h.b1, m), __fmul_rn(h.omb1, g));
+	v = __fadd_rn(__fmul_rn(h.b2, v), __fmul_rn(__fmul_rn(h.omb2, g), g));
 	adam_apply(a, lrwd, p, m, v);
 }
 
@@ -106,7 +112,7 @@ __device__ __forceinline__ void q8_scale(uint32_t amax_bits, float top, float &s
 	const bool none = amax < 7.8886090522101181e-31f;	/* 2^-100 */
 
 	scale = none ? 0.0f : __fdiv_rn(amax, top);
-	inv = none ? 0.0f : __fdiv_rn(top, amax);
+	inv = none ? 0.0f : __fmul_rn(__frcp_rn(amax), top);
 }
 
 __device__ __forceinline__ float e4m3_to_float(uint32_t c)
@@ -127,6 +133,25 @@ __device__ __forceinline__ uint32_t to_e4m3(float x)
 __device__ __forceinline__ uint32_t to_e5m2(float x)
 {
 	return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E5M2);
+}
+
+/*
+** New moments of element i of a block over their scales, as the numbers to code: x by the multiplier, rounded by
+** chance if asked for, and a v that is not zero at least the smallest number (its conversion rounds to nearest).
+*/
+__device__ __forceinline__ void q8_round(bool random, uint32_t key, uint32_t i, float mi, float vi, float &m, float &v)
+{
+	float x = __fmul_rn(m, mi);
+	float y = __fmul_rn(v, vi);
+
+	if (random) {
+		const uint32_t r = mix32(key + i * 0x9e3779b9u);
+
+		x = stochastic<3>(x, r & 0xffffu, 0.015625f);		/* 2^-6 */
+		y = stochastic<2>(y, r >> 16, 6.103515625e-5f);		/* 2^-14 */
+	}
+	m = x;
+	v = v > 0.0f && vi > 0.0f ? fmaxf(y, 1.52587890625e-5f) : y;	/* 2^-16 */
 }
 
 /* ---- one warp's run of at most 256 elements -------------------------------------- */
@@ -201,23 +226,12 @@ __device__ __forceinline__ void run_scalar(const mt_launch &a, const mt_desc &d,
 #pragma unroll
 		for (int j = 0; j < 8; j++) {
 			const int i = j * 32 + lane;
-			float x = m[j] * mi;
-			float y = v[j] * vi;
-			uint32_t c;
 
 			if (i >= len)
 				continue;
-			if (a.la.flags & ANNI_STEP_STOCHASTIC) {
-				const uint32_t r = mix32(key + (uint32_t)i * 0x9e3779b9u);
-
-				x = stochastic<3>(x, r & 0xffffu, 0.015625f);
-				y = stochastic<2>(y, r >> 16, 6.103515625e-5f);
-			}
-			static_cast<uint8_t *>(d.m)[e0 + i] = (uint8_t)to_e4m3(x);
-			c = to_e5m2(y);
-			if (c == 0 && v[j] > 0.0f && vi > 0.0f)
-				c = 1;
-			static_cast<uint8_t *>(d.v)[e0 + i] = (uint8_t)c;
+			q8_round(a.la.flags & ANNI_STEP_STOCHASTIC, key, (uint32_t)i, mi, vi, m[j], v[j]);
+			static_cast<uint8_t *>(d.m)[e0 + i] = (uint8_t)to_e4m3(m[j]);
+			static_cast<uint8_t *>(d.v)[e0 + i] = (uint8_t)to_e5m2(v[j]);
 		}
 	}
 	if (a.la.flags & ANNI_STEP_ZERO_GRAD)
@@ -225,41 +239,204 @@ __device__ __forceinline__ void run_scalar(const mt_launch &a, const mt_desc &d,
 			io8<GradT>::store1(grad, e0 + i, 0.0f);
 }
 
-/* where tile t lies for this warp: tensor, first element of the run, its length (0: nothing) */
-__device__ __forceinline__ uint32_t run_of(const mt_launch &a, uint32_t t, int64_t &e0, int &len)
+/*
+** A whole run on aligned addresses: lane l holds elements 4 l .. 4 l + 3 of each half, so every access of the
+** warp is one contiguous piece (512 bytes of fp32, 128 of codes).
+*/
+template <typename GradT>
+__device__ __forceinline__ void run_vec_f32(const mt_launch &a, const mt_desc &d, void *grad, int64_t e0, double coef)
 {
-	const uint32_t s = a.tile_of[t];
-	const int64_t left = a.desc[s].n
-	    - (e0 = (int64_t)(t - a.desc[s].tile0) * ANNI_MT_TILE + (threadIdx.x >> 5) * ANNI_MT_BLOCK);
+	const float lrwd = d.wd ? a.la.lrwd : 0.0f;
 
-	len = left <= 0 ? 0 : left < ANNI_MT_BLOCK ? (int)left : ANNI_MT_BLOCK;
-	return s;
+#pragma unroll 1
+	for (int k = 0; k < 2; k++) {
+		const uint64_t e = (uint64_t)e0 + 128 * k + (threadIdx.x & 31) * 4;
+		const f32x4 g = io4<GradT>::load(grad, e);
+		f32x4 p = io4<float>::load(d.p, e);
+		f32x4 m = io4<float>::load(d.m, e);
+		f32x4 v = io4<float>::load(d.v, e);
+
+#pragma unroll
+		for (int j = 0; j < 4; j++)
+			adam_elem<false>(a.la, coef, lrwd, g.x[j], p.x[j], m.x[j], v.x[j]);
+		io4<float>::store(d.p, e, p);
+		io4<float>::store(d.m, e, m);
+		io4<float>::store(d.v, e, v);
+		if (d.twin)
+			io4<__nv_bfloat16>::store(d.twin, e, p);
+		if (a.la.flags & ANNI_STEP_ZERO_GRAD)
+			io4<GradT>::zero(grad, e);
+	}
 }
 
+template <__nv_fp8_interpretation_t KIND>
+__device__ __forceinline__ f32x4 decode4(uint32_t q, float scale)
+{
+	const float2 lo = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(q & 0xffffu), KIND)));
+	const float2 hi = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(q >> 16), KIND)));
+	f32x4 r;
+
+	r.x[0] = __fmul_rn(lo.x, scale);
+	r.x[1] = __fmul_rn(lo.y, scale);
+	r.x[2] = __fmul_rn(hi.x, scale);
+	r.x[3] = __fmul_rn(hi.y, scale);
+	return r;
+}
+
+template <__nv_fp8_interpretation_t KIND>
+__device__ __forceinline__ uint32_t encode4(const f32x4 &y)
+{
+	return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(y.x[0], y.x[1]), __NV_SATFINITE, KIND)
+	    | ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(y.x[2], y.x[3]), __NV_SATFINITE, KIND) << 16);
+}
+
+template <typename GradT>
+__device__ __forceinline__ void run_vec_q8(const mt_launch &a, const mt_desc &d, void *grad, int64_t e0,
+	const q8_hyper &h)
+{
+	const int lane = threadIdx.x & 31;
+	const float lrwd = d.wd ? a.la.lrwd : 0.0f;
+	const int64_t blk = e0 / ANNI_MT_BLOCK;
+	const uint64_t e = (uint64_t)e0 + lane * 4;
+	f32x4 g[2];
+	f32x4 p[2];
+	f32x4 m[2];
+	f32x4 v[2];
+	uint32_t qm[2];
+	uint32_t qv[2];
+	float ms;
+	float vs;
+	float mi;
+	float vi;
+	uint32_t am = 0;
+	uint32_t av = 0;
+
+#pragma unroll
+	for (int k = 0; k < 2; k++) {
+		g[k] = io4<GradT>::load(grad, e + 128 * k);
+		p[k] = io4<float>::load(d.p, e + 128 * k);
+		qm[k] = __ldcs(reinterpret_cast<const uint32_t *>(static_cast<const uint8_t *>(d.m) + e + 128 * k));
+		qv[k] = __ldcs(reinterpret_cast<const uint32_t *>(static_cast<const uint8_t *>(d.v) + e + 128 * k));
+	}
+	ms = d.ms[blk];
+	vs = d.vs[blk];
+#pragma unroll
+	for (int k = 0; k < 2; k++) {
+		m[k] = decode4<__NV_E4M3>(qm[k], ms);
+		v[k] = decode4<__NV_E5M2>(qv[k], vs);
+#pragma unroll
+		for (int j = 0; j < 4; j++) {
+			adam_q8(a.la, h, lrwd, g[k].x[j], p[k].x[j], m[k].x[j], v[k].x[j]);
+			am = max(am, __float_as_uint(fabsf(m[k].x[j])));
+			av = max(av, __float_as_uint(v[k].x[j]));
+		}
+		io4<float>::store(d.p, e + 128 * k, p[k]);
+		if (d.twin)
+			io4<__nv_bfloat16>::store(d.twin, e + 128 * k, p[k]);
+		if (a.la.flags & ANNI_STEP_ZERO_GRAD)
+			io4<GradT>::zero(grad, e + 128 * k);
+	}
+	am = __reduce_max_sync(0xffffffffu, am);
+	av = __reduce_max_sync(0xffffffffu, av);
+	q8_scale(am, 448.0f, ms, mi);
+	q8_scale(av, 57344.0f, vs, vi);
+	if (lane == 0) {
+		d.ms[blk] = ms;
+		d.vs[blk] = vs;
+	}
+	const bool random = a.la.flags & ANNI_STEP_STOCHASTIC;
+	const uint32_t key = random ? block_key(a.seed, d.block0 + (uint64_t)blk) : 0;
+
+#pragma unroll
+	for (int k = 0; k < 2; k++) {
+#pragma unroll
+		for (int j = 0; j < 4; j++)
+			q8_round(random, key, (uint32_t)(128 * k + lane * 4 + j), mi, vi, m[k].x[j], v[k].x[j]);
+		__stcs(reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(d.m) + e + 128 * k), encode4<__NV_E4M3>(m[k]));
+		__stcs(reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(d.v) + e + 128 * k), encode4<__NV_E5M2>(v[k]));
+	}
+}
+
+template <typename GradT, bool Q8>
+__device__ __forceinline__ void mt_update_phase(const mt_launch &a, const decision &dec, const q8_hyper &h)
+{
+	const int64_t warp0 = (threadIdx.x >> 5) * ANNI_MT_BLOCK;
+
+	/* backwards: the gradients read last by the norm phase are the likeliest to sit in L2 */
+	for (uint32_t r = (a.tiles + gridDim.x - 1) / gridDim.x; r > 0; r--) {
+		const uint32_t t = (r - 1) * gridDim.x + blockIdx.x;
+
+		if (t >= a.tiles)
+			continue;
+		const uint32_t s = a.tile_of[t];
+		void *grad = a.grad[s];
+		const mt_desc &d = a.desc[s];
+		const int64_t n = d.n;
+		const bool vec = d.vec && ((uintptr_t)grad & 15) == 0 && !dec.skip;
+		int64_t e0 = (int64_t)(t - d.tile0) * ANNI_MT_TILE + warp0;
+
+		if (!grad)
+			continue;
+#pragma unroll 1
+		for (int k = 0; k < ANNI_MT_TILE / ANNI_MT_PASS && e0 < n; k++, e0 += ANNI_MT_PASS) {
+			const int64_t left = n - e0;
+
+			if (vec && left >= ANNI_MT_BLOCK) {
+				if (Q8)
+					run_vec_q8<GradT>(a, d, grad, e0, h);
+				else
+					run_vec_f32<GradT>(a, d, grad, e0, dec.coef);
+			} else
+				run_scalar<GradT, Q8>(a, d, grad, e0, left < ANNI_MT_BLOCK ? (int)left : ANNI_MT_BLOCK,
+				    dec.coef, h, dec.skip);
+		}
+	}
+}
+
+/*
+** Sum of squares: a warp takes a tile, so that each lane has several 16-byte loads in flight for one look
+** at the tables.
+*/
 template <typename GradT>
 __device__ __forceinline__ double mt_norm_phase(const mt_launch &a)
 {
 	const int lane = threadIdx.x & 31;
-	double acc = 0.0;
+	const uint32_t step = gridDim.x * (ANNI_THREADS / 32);
+	double acc0 = 0.0;
+	double acc1 = 0.0;
 
-	for (uint32_t t = blockIdx.x; t < a.tiles; t += gridDim.x) {
-		int64_t e0;
-		int len;
-		const void *grad = a.grad[run_of(a, t, e0, len)];
+	for (uint32_t t = (threadIdx.x >> 5) * gridDim.x + blockIdx.x; t < a.tiles; t += step) {
+		const uint32_t s = a.tile_of[t];
+		const void *grad = a.grad[s];
+		const int64_t lo = (int64_t)(t - a.desc[s].tile0) * ANNI_MT_TILE;
+		const int64_t left = a.desc[s].n - lo;
+		const int len = left < ANNI_MT_TILE ? (int)left : ANNI_MT_TILE;
+		int i = 0;
 
 		if (!grad)
 			continue;
-		for (int i = lane; i < len; i += 32) {
-			const double g = (double)io8<GradT>::load1(grad, e0 + i);
+		if (((uintptr_t)grad & 15) == 0)
+			for (; i + 1024 <= len; i += 1024) {
+				f32x8 g[4];
 
-			acc = fma(g, g, acc);
+#pragma unroll
+				for (int k = 0; k < 4; k++)
+					g[k] = io8<GradT>::load_keep(grad, (uint64_t)lo + i + 256 * k + lane * 8);
+#pragma unroll
+				for (int k = 0; k < 4; k++)
+					norm_accumulate<GradT>(g[k], acc0, acc1);
+			}
+		for (i += lane; i < len; i += 32) {
+			const double g = (double)io8<GradT>::load1(grad, (uint64_t)lo + i);
+
+			acc0 = fma(g, g, acc0);
 		}
 	}
-	return acc;
+	return acc0 + acc1;
 }
 
 template <typename GradT, bool Q8>
-__global__ void __launch_bounds__(ANNI_THREADS) mt_step_kernel(const mt_launch a)
+__global__ void __launch_bounds__(ANNI_THREADS, 4) mt_step_kernel(const mt_launch a)
 {
 	decision d;
 	q8_hyper h;
@@ -288,15 +465,7 @@ __global__ void __launch_bounds__(ANNI_THREADS) mt_step_kernel(const mt_launch a
 	h.omb2 = (float)a.la.omb2;
 	h.coef = (float)d.coef;
 	if (!d.skip || (a.la.flags & ANNI_STEP_ZERO_GRAD))
-		for (uint32_t t = blockIdx.x; t < a.tiles; t += gridDim.x) {
-			int64_t e0;
-			int len;
-			const uint32_t s = run_of(a, t, e0, len);
-			void *grad = a.grad[s];
-
-			if (grad && len > 0)
-				run_scalar<GradT, Q8>(a, a.desc[s], grad, e0, len, d.coef, h, d.skip);
-		}
+		mt_update_phase<GradT, Q8>(a, d, h);
 	step_epilogue(a.la.ctl, d.skip);
 }
 
@@ -339,6 +508,14 @@ bool overlapping(const std::vector<range> &v)
 		if (v[k - 1].hi > v[k].lo)
 			return true;
 	return false;
+}
+
+/* 16-byte accesses of fp32, 8-byte of twins, 4-byte of codes */
+bool aligned(const mt_desc &d, bool q8)
+{
+	const uintptr_t mv = (uintptr_t)d.m | (uintptr_t)d.v;
+
+	return (((uintptr_t)d.p | (q8 ? 0 : mv)) & 15) == 0 && (mv & 3) == 0 && ((uintptr_t)d.twin & 7) == 0;
 }
 
 /* the handle's device for the length of a call */
@@ -460,7 +637,8 @@ static int create(const anni_mt_tensor *list, int n, anni_mtstep *h)
 		grads[i] = list[i].grad;
 		desc[i] = { list[i].param, list[i].m, list[i].v, list[i].m_scale, list[i].v_scale,
 		    (list[i].flags & ANNI_SEG_TWIN_BF16) ? (uint16_t *)list[i].twin_bf16 : NULL, list[i].n, block0,
-		    (uint32_t)tiles, (list[i].flags & ANNI_SEG_WD) ? 1u : 0u };
+		    (uint32_t)tiles, (uint16_t)((list[i].flags & ANNI_SEG_WD) ? 1 : 0), 0 };
+		desc[i].vec = aligned(desc[i], h->state_dtype == ANNI_DT_Q8);
 		tiles += (uint64_t)(list[i].n + ANNI_MT_TILE - 1) / ANNI_MT_TILE;
 		block0 += (uint64_t)(list[i].n + ANNI_MT_BLOCK - 1) / ANNI_MT_BLOCK;
 		if (tiles > 0x7fffffffu)
