@@ -20,8 +20,7 @@
 #include "optstep_internal.h"
 #include "optstep_device.h"
 
-#define ANNI_MT_PASS		(ANNI_THREADS / 32 * ANNI_MT_BLOCK)	/* elements a block takes at once */
-#define ANNI_MT_TILE		(2 * ANNI_MT_PASS)
+#define ANNI_MT_TILE		(ANNI_THREADS / 32 * ANNI_MT_BLOCK)	/* elements a block takes at once */
 #define ANNI_MT_ADDRS		448	/* gradient addresses per launch of set_grads_kernel */
 
 namespace {
@@ -41,6 +40,8 @@ struct mt_desc {
 	uint16_t	vec;		/* everything but the gradient on the alignment of the vector accesses */
 };
 
+static_assert(sizeof(mt_desc) % 8 == 0, "mt_held keeps the gradient's address behind it");
+
 struct mt_launch {
 	anni_launch	la;		/* hyper-parameters, flags, control block */
 	const mt_desc	*desc;
@@ -48,6 +49,10 @@ struct mt_launch {
 	const uint32_t	*tile_of;	/* tensor of each tile */
 	uint32_t	tiles;
 	uint64_t	seed;
+	float		b1;		/* beta1, 1 - beta1, beta2, 1 - beta2 for the 8-bit form */
+	float		omb1;
+	float		b2;
+	float		omb2;
 };
 
 /* ---- 8-bit moments ------------------------------------------------------------ */
@@ -67,7 +72,7 @@ __device__ __forceinline__ uint32_t block_key(uint64_t seed, uint64_t block)
 }
 
 /*
-** x to KEPT bits of mantissa, up with the probability of the part cut off: 16 random bits are added to
+** x >= 0 to KEPT bits of mantissa, up with the probability of the part cut off: 16 random bits are added to
 ** the top of the bits that go, and the carry decides.  Below LEAST, the smallest normal number of the
 ** 8-bit type, its numbers are equally spaced; adding LEAST puts x into the binade with that spacing.
 */
@@ -75,34 +80,76 @@ template <int KEPT>
 __device__ __forceinline__ float stochastic(float x, uint32_t r16, float least)
 {
 	const int cut = 23 - KEPT;
-	const float a = fabsf(x);
-	const float add = a < least ? least : 0.0f;
-	const uint32_t bits = __float_as_uint(__fadd_rn(a, add)) + (r16 << (cut - 16));
-	const float r = __fsub_rn(__uint_as_float(bits >> cut << cut), add);
+	const float add = x < least ? least : 0.0f;
+	const uint32_t bits = __float_as_uint(__fadd_rn(x, add)) + (r16 << (cut - 16));
 
-	return copysignf(r, x);
+	return __fsub_rn(__uint_as_float(bits >> cut << cut), add);
 }
 
-struct q8_hyper {
-	float	b1;
-	float	omb1;
-	float	b2;
-	float	omb2;
-	float	coef;
-};
+/* two floats in one instruction each, every result rounded on its own */
+typedef unsigned long long f32x2;
+
+__device__ __forceinline__ f32x2 pair(float lo, float hi)
+{
+	f32x2 r;
+
+	asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+	return r;
+}
+
+__device__ __forceinline__ void unpair(f32x2 x, float &lo, float &hi)
+{
+	asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x));
+}
+
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b)
+{
+	f32x2 r;
+
+	asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+	return r;
+}
+
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b)
+{
+	f32x2 r;
+
+	asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+	return r;
+}
+
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c)
+{
+	f32x2 r;
+
+	asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+	return r;
+}
 
 /*
-** Moments in float (their stored form has three and two bits of mantissa), every product and sum rounded on its
-** own, so that a float restatement of the formula lands on the same codes; then the shared parameter update.
+** Two elements of the 8-bit form.  Moments in float (their stored form has three and two bits of mantissa),
+** every product and sum rounded on its own, so that a float restatement of the formula lands on the same codes;
+** then the parameter update of adam_apply, operation for operation.
 */
-__device__ __forceinline__ void adam_q8(const anni_launch &a, const q8_hyper &h, float lrwd, float gf, float &p,
-	float &m, float &v)
+__device__ __forceinline__ void adam_q8(const mt_launch &a, float coef, float lrwd, float g0, float g1, float &p0,
+	float &p1, f32x2 &m, f32x2 &v)
 {
-	const float g = __fmul_rn(gf, h.coef);
+	const f32x2 g = mul2(pair(g0, g1), pair(coef, coef));
+	f32x2 p = pair(p0, p1);
+	float s0;
+	float s1;
+	float d0;
+	float d1;
 
-	m = __fadd_rn(__fmul_rn(h.b1, m), __fmul_rn(h.omb1, g));
-	v = __fadd_rn(__fmul_rn(h.b2, v), __fmul_rn(__fmul_rn(h.omb2, g), g));
-	adam_apply(a, lrwd, p, m, v);
+	m = add2(mul2(pair(a.b1, a.b1), m), mul2(pair(a.omb1, a.omb1), g));
+	v = add2(mul2(pair(a.b2, a.b2), v), mul2(mul2(pair(a.omb2, a.omb2), g), g));
+	unpair(mul2(v, pair(a.la.ibc2_s24, a.la.ibc2_s24)), s0, s1);
+	unpair(fma2(pair(sqrt_approx_ftz(s0), sqrt_approx_ftz(s1)), pair(268435456.0f, 268435456.0f),
+	    pair(a.la.eps_s40, a.la.eps_s40)), d0, d1);
+	p = fma2(mul2(mul2(pair(a.la.lrbc1_s40, a.la.lrbc1_s40), m), pair(rcp_approx_ftz(d0), rcp_approx_ftz(d1))),
+	    pair(-1.0f, -1.0f), p);
+	p = fma2(pair(-lrwd, -lrwd), p, p);
+	unpair(p, p0, p1);
 }
 
 /* scale of a block from its largest value (as bits, >= 0) and the multiplier that undoes it; a NaN stays one */
@@ -136,33 +183,31 @@ __device__ __forceinline__ uint32_t to_e5m2(float x)
 }
 
 /*
-** New moments of element i of a block over their scales, as the numbers to code: x by the multiplier, rounded by
-** chance if asked for, and a v that is not zero at least the smallest number (its conversion rounds to nearest).
+** What is coded for element i of a block, from its new moments over their scales x and y: rounded by chance if
+** asked for, and y at least the smallest number unless v is zero (the conversions round to nearest).
 */
-__device__ __forceinline__ void q8_round(bool random, uint32_t key, uint32_t i, float mi, float vi, float &m, float &v)
+__device__ __forceinline__ void q8_round(bool random, uint32_t key, uint32_t i, float v, float vi, float &x, float &y)
 {
-	float x = __fmul_rn(m, mi);
-	float y = __fmul_rn(v, vi);
-
 	if (random) {
 		const uint32_t r = mix32(key + i * 0x9e3779b9u);
 
-		x = stochastic<3>(x, r & 0xffffu, 0.015625f);		/* 2^-6 */
+		x = copysignf(stochastic<3>(fabsf(x), r & 0xffffu, 0.015625f), x);	/* 2^-6 */
 		y = stochastic<2>(y, r >> 16, 6.103515625e-5f);		/* 2^-14 */
 	}
-	m = x;
-	v = v > 0.0f && vi > 0.0f ? fmaxf(y, 1.52587890625e-5f) : y;	/* 2^-16 */
+	if (v > 0.0f && vi > 0.0f)
+		y = fmaxf(y, 1.52587890625e-5f);	/* 2^-16 */
 }
 
 /* ---- one warp's run of at most 256 elements -------------------------------------- */
 
 /*
-** Element-wise: lane l holds elements l, l + 32, ... of the run, so plain accesses coalesce whatever
-** the address.
+** Tensors on addresses that only their type allows: element-wise, lane l on elements l, l + 32, ... of the
+** run, so that plain accesses coalesce.  One element at a time, which keeps its registers out of the way of the
+** vector path's.
 */
 template <typename GradT, bool Q8>
 __device__ __forceinline__ void run_scalar(const mt_launch &a, const mt_desc &d, void *grad, int64_t e0, int len,
-	double coef, const q8_hyper &h, bool skip)
+	double coef, bool skip)
 {
 	const int lane = threadIdx.x & 31;
 	const float lrwd = d.wd ? a.la.lrwd : 0.0f;
@@ -190,9 +235,13 @@ __device__ __forceinline__ void run_scalar(const mt_launch &a, const mt_desc &d,
 				const float g = io8<GradT>::load1(grad, e);
 
 				if (Q8) {
-					m[j] = e4m3_to_float(static_cast<const uint8_t *>(d.m)[e]) * ms;
-					v[j] = e5m2_to_float(static_cast<const uint8_t *>(d.v)[e]) * vs;
-					adam_q8(a.la, h, lrwd, g, p, m[j], v[j]);
+					f32x2 m2 = pair(__fmul_rn(e4m3_to_float(static_cast<const uint8_t *>(d.m)[e]), ms), 0.0f);
+					f32x2 v2 = pair(__fmul_rn(e5m2_to_float(static_cast<const uint8_t *>(d.v)[e]), vs), 0.0f);
+					float none = 0.0f;
+
+					adam_q8(a, (float)coef, lrwd, g, 0.0f, p, none, m2, v2);
+					unpair(m2, m[j], none);
+					unpair(v2, v[j], none);
 					am = max(am, __float_as_uint(fabsf(m[j])));
 					av = max(av, __float_as_uint(v[j]));
 				} else {
@@ -229,9 +278,12 @@ __device__ __forceinline__ void run_scalar(const mt_launch &a, const mt_desc &d,
 
 			if (i >= len)
 				continue;
-			q8_round(a.la.flags & ANNI_STEP_STOCHASTIC, key, (uint32_t)i, mi, vi, m[j], v[j]);
-			static_cast<uint8_t *>(d.m)[e0 + i] = (uint8_t)to_e4m3(m[j]);
-			static_cast<uint8_t *>(d.v)[e0 + i] = (uint8_t)to_e5m2(v[j]);
+			float x = __fmul_rn(m[j], mi);
+			float y = __fmul_rn(v[j], vi);
+
+			q8_round(a.la.flags & ANNI_STEP_STOCHASTIC, key, (uint32_t)i, v[j], vi, x, y);
+			static_cast<uint8_t *>(d.m)[e0 + i] = (uint8_t)to_e4m3(x);
+			static_cast<uint8_t *>(d.v)[e0 + i] = (uint8_t)to_e5m2(y);
 		}
 	}
 	if (a.la.flags & ANNI_STEP_ZERO_GRAD)
@@ -240,68 +292,138 @@ __device__ __forceinline__ void run_scalar(const mt_launch &a, const mt_desc &d,
 }
 
 /*
-** A whole run on aligned addresses: lane l holds elements 4 l .. 4 l + 3 of each half, so every access of the
+** The same on elements e .. e + 3 of which the first `left` exist (ALL: four do); what does not exist reads as
+** zero.  Only the last lane with elements of a tensor takes the element-wise road.
+*/
+template <typename T, bool ALL>
+__device__ __forceinline__ f32x4 load_some(const void *base, uint64_t e, int left)
+{
+	f32x4 r;
+
+	if (ALL || left >= 4)
+		return io4<T>::load(base, e);
+#pragma unroll
+	for (int j = 0; j < 4; j++)
+		r.x[j] = j < left ? io8<T>::load1(base, e + j) : 0.0f;
+	return r;
+}
+
+template <typename T, bool ALL>
+__device__ __forceinline__ void store_some(void *base, uint64_t e, const f32x4 &r, int left)
+{
+	if (ALL || left >= 4) {
+		io4<T>::store(base, e, r);
+		return;
+	}
+#pragma unroll
+	for (int j = 0; j < 4; j++)
+		if (j < left)
+			io8<T>::store1(base, e + j, r.x[j]);
+}
+
+template <bool ALL>
+__device__ __forceinline__ uint32_t load_codes(const void *base, uint64_t e, int left)
+{
+	const uint8_t *p = static_cast<const uint8_t *>(base) + e;
+	uint32_t q = 0;
+
+	if (ALL || left >= 4)
+		return __ldcs(reinterpret_cast<const uint32_t *>(p));
+#pragma unroll
+	for (int j = 0; j < 4; j++)
+		if (j < left)
+			q |= (uint32_t)p[j] << (8 * j);
+	return q;
+}
+
+template <bool ALL>
+__device__ __forceinline__ void store_codes(void *base, uint64_t e, uint32_t q, int left)
+{
+	uint8_t *p = static_cast<uint8_t *>(base) + e;
+
+	if (ALL || left >= 4) {
+		__stcs(reinterpret_cast<uint32_t *>(p), q);
+		return;
+	}
+#pragma unroll
+	for (int j = 0; j < 4; j++)
+		if (j < left)
+			p[j] = (uint8_t)(q >> (8 * j));
+}
+
+/*
+** A run of len elements on aligned addresses: lane l holds elements 4 l .. 4 l + 3 of each half, so every access of the
 ** warp is one contiguous piece (512 bytes of fp32, 128 of codes).
 */
-template <typename GradT>
-__device__ __forceinline__ void run_vec_f32(const mt_launch &a, const mt_desc &d, void *grad, int64_t e0, double coef)
+template <typename GradT, bool ALL>
+__device__ __forceinline__ void run_vec_f32(const mt_launch &a, const mt_desc &d, void *grad, int64_t e0, int len,
+	double coef)
 {
 	const float lrwd = d.wd ? a.la.lrwd : 0.0f;
+	float *const pp = d.p;		/* copies: the compiler cannot know that the stores leave d alone */
+	void *const mp = d.m;
+	void *const vp = d.v;
+	uint16_t *const tp = d.twin;
 
 #pragma unroll 1
 	for (int k = 0; k < 2; k++) {
-		const uint64_t e = (uint64_t)e0 + 128 * k + (threadIdx.x & 31) * 4;
-		const f32x4 g = io4<GradT>::load(grad, e);
-		f32x4 p = io4<float>::load(d.p, e);
-		f32x4 m = io4<float>::load(d.m, e);
-		f32x4 v = io4<float>::load(d.v, e);
+		const int i = 128 * k + (threadIdx.x & 31) * 4;
+		const int left = len - i;
+		const uint64_t e = (uint64_t)e0 + i;
+
+		if (!ALL && left <= 0)
+			break;
+		const f32x4 g = load_some<GradT, ALL>(grad, e, left);
+		f32x4 p = load_some<float, ALL>(pp, e, left);
+		f32x4 m = load_some<float, ALL>(mp, e, left);
+		f32x4 v = load_some<float, ALL>(vp, e, left);
 
 #pragma unroll
 		for (int j = 0; j < 4; j++)
 			adam_elem<false>(a.la, coef, lrwd, g.x[j], p.x[j], m.x[j], v.x[j]);
-		io4<float>::store(d.p, e, p);
-		io4<float>::store(d.m, e, m);
-		io4<float>::store(d.v, e, v);
-		if (d.twin)
-			io4<__nv_bfloat16>::store(d.twin, e, p);
+		store_some<float, ALL>(pp, e, p, left);
+		store_some<float, ALL>(mp, e, m, left);
+		store_some<float, ALL>(vp, e, v, left);
+		if (tp)
+			store_some<__nv_bfloat16, ALL>(tp, e, p, left);
 		if (a.la.flags & ANNI_STEP_ZERO_GRAD)
-			io4<GradT>::zero(grad, e);
+			store_some<GradT, ALL>(grad, e, f32x4{}, left);
 	}
 }
 
 template <__nv_fp8_interpretation_t KIND>
-__device__ __forceinline__ f32x4 decode4(uint32_t q, float scale)
+__device__ __forceinline__ f32x2 decode2(uint32_t q, float scale)
 {
-	const float2 lo = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(q & 0xffffu), KIND)));
-	const float2 hi = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(q >> 16), KIND)));
-	f32x4 r;
+	const float2 x = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)q, KIND)));
 
-	r.x[0] = __fmul_rn(lo.x, scale);
-	r.x[1] = __fmul_rn(lo.y, scale);
-	r.x[2] = __fmul_rn(hi.x, scale);
-	r.x[3] = __fmul_rn(hi.y, scale);
-	return r;
+	return mul2(pair(x.x, x.y), pair(scale, scale));
 }
 
 template <__nv_fp8_interpretation_t KIND>
-__device__ __forceinline__ uint32_t encode4(const f32x4 &y)
+__device__ __forceinline__ uint32_t encode2(float lo, float hi)
 {
-	return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(y.x[0], y.x[1]), __NV_SATFINITE, KIND)
-	    | ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(y.x[2], y.x[3]), __NV_SATFINITE, KIND) << 16);
+	return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, KIND);
 }
 
-template <typename GradT>
+/*
+** WHOLE: the block's eight warps are on the eight runs of a whole tile, block-uniformly; their new scales are
+** then stored by one warp, two full 32-byte sectors, instead of by each warp, four bytes twice.  Single-lane
+** stores into sectors that other warps load at the same time cost a quarter of the step (184.7 M elements
+** without arithmetic: 574 us against 447 us without those stores; 474 us this way).
+*/
+template <typename GradT, bool WHOLE>
 __device__ __forceinline__ void run_vec_q8(const mt_launch &a, const mt_desc &d, void *grad, int64_t e0,
-	const q8_hyper &h)
+	int len, float coef, float (*slot)[ANNI_THREADS / 32])
 {
 	const int lane = threadIdx.x & 31;
 	const float lrwd = d.wd ? a.la.lrwd : 0.0f;
 	const int64_t blk = e0 / ANNI_MT_BLOCK;
 	const uint64_t e = (uint64_t)e0 + lane * 4;
+	const int left = len - lane * 4;	/* of this lane's four, and 128 more than of its second four */
 	f32x4 g[2];
 	f32x4 p[2];
-	f32x4 m[2];
-	f32x4 v[2];
+	f32x2 m[4];
+	f32x2 v[4];
 	uint32_t qm[2];
 	uint32_t qv[2];
 	float ms;
@@ -313,34 +435,53 @@ __device__ __forceinline__ void run_vec_q8(const mt_launch &a, const mt_desc &d,
 
 #pragma unroll
 	for (int k = 0; k < 2; k++) {
-		g[k] = io4<GradT>::load(grad, e + 128 * k);
-		p[k] = io4<float>::load(d.p, e + 128 * k);
-		qm[k] = __ldcs(reinterpret_cast<const uint32_t *>(static_cast<const uint8_t *>(d.m) + e + 128 * k));
-		qv[k] = __ldcs(reinterpret_cast<const uint32_t *>(static_cast<const uint8_t *>(d.v) + e + 128 * k));
+		g[k] = load_some<GradT, WHOLE>(grad, e + 128 * k, left - 128 * k);
+		p[k] = load_some<float, WHOLE>(d.p, e + 128 * k, left - 128 * k);
+		qm[k] = load_codes<WHOLE>(d.m, e + 128 * k, left - 128 * k);
+		qv[k] = load_codes<WHOLE>(d.v, e + 128 * k, left - 128 * k);
 	}
 	ms = d.ms[blk];
 	vs = d.vs[blk];
 #pragma unroll
 	for (int k = 0; k < 2; k++) {
-		m[k] = decode4<__NV_E4M3>(qm[k], ms);
-		v[k] = decode4<__NV_E5M2>(qv[k], vs);
 #pragma unroll
-		for (int j = 0; j < 4; j++) {
-			adam_q8(a.la, h, lrwd, g[k].x[j], p[k].x[j], m[k].x[j], v[k].x[j]);
-			am = max(am, __float_as_uint(fabsf(m[k].x[j])));
-			av = max(av, __float_as_uint(v[k].x[j]));
+		for (int j = 0; j < 2; j++) {
+			f32x2 &mm = m[2 * k + j];
+			f32x2 &vv = v[2 * k + j];
+			float lo;
+			float hi;
+
+			mm = decode2<__NV_E4M3>((qm[k] >> (16 * j)) & 0xffffu, ms);
+			vv = decode2<__NV_E5M2>((qv[k] >> (16 * j)) & 0xffffu, vs);
+			adam_q8(a, coef, lrwd, g[k].x[2 * j], g[k].x[2 * j + 1], p[k].x[2 * j], p[k].x[2 * j + 1], mm, vv);
+			unpair(mm, lo, hi);
+			am = max(am, max(__float_as_uint(fabsf(lo)), __float_as_uint(fabsf(hi))));
+			unpair(vv, lo, hi);
+			av = max(av, max(__float_as_uint(lo), __float_as_uint(hi)));
 		}
-		io4<float>::store(d.p, e + 128 * k, p[k]);
+		store_some<float, WHOLE>(d.p, e + 128 * k, p[k], left - 128 * k);
 		if (d.twin)
-			io4<__nv_bfloat16>::store(d.twin, e + 128 * k, p[k]);
+			store_some<__nv_bfloat16, WHOLE>(d.twin, e + 128 * k, p[k], left - 128 * k);
 		if (a.la.flags & ANNI_STEP_ZERO_GRAD)
-			io4<GradT>::zero(grad, e + 128 * k);
+			store_some<GradT, WHOLE>(grad, e + 128 * k, f32x4{}, left - 128 * k);
 	}
 	am = __reduce_max_sync(0xffffffffu, am);
 	av = __reduce_max_sync(0xffffffffu, av);
 	q8_scale(am, 448.0f, ms, mi);
 	q8_scale(av, 57344.0f, vs, vi);
-	if (lane == 0) {
+	if (WHOLE) {
+		const int w = threadIdx.x >> 5;
+
+		/* the caller alternates two slots: one barrier per tile keeps writers and the reader apart */
+		if (lane == 0) {
+			slot[0][w] = ms;
+			slot[1][w] = vs;
+		}
+		__syncthreads();
+		if (w == 0 && lane < 2 * (ANNI_THREADS / 32))
+			(lane < ANNI_THREADS / 32 ? d.ms : d.vs)[blk + (lane & (ANNI_THREADS / 32 - 1))] =
+			    slot[lane / (ANNI_THREADS / 32)][lane & (ANNI_THREADS / 32 - 1)];
+	} else if (lane == 0) {
 		d.ms[blk] = ms;
 		d.vs[blk] = vs;
 	}
@@ -349,46 +490,124 @@ __device__ __forceinline__ void run_vec_q8(const mt_launch &a, const mt_desc &d,
 
 #pragma unroll
 	for (int k = 0; k < 2; k++) {
+		uint32_t cm = 0;
+		uint32_t cv = 0;
+
 #pragma unroll
-		for (int j = 0; j < 4; j++)
-			q8_round(random, key, (uint32_t)(128 * k + lane * 4 + j), mi, vi, m[k].x[j], v[k].x[j]);
-		__stcs(reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(d.m) + e + 128 * k), encode4<__NV_E4M3>(m[k]));
-		__stcs(reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(d.v) + e + 128 * k), encode4<__NV_E5M2>(v[k]));
+		for (int j = 0; j < 2; j++) {
+			const uint32_t i = (uint32_t)(128 * k + lane * 4 + 2 * j);
+			float x0;
+			float x1;
+			float y0;
+			float y1;
+			float v0;
+			float v1;
+
+			unpair(mul2(m[2 * k + j], pair(mi, mi)), x0, x1);
+			unpair(mul2(v[2 * k + j], pair(vi, vi)), y0, y1);
+			unpair(v[2 * k + j], v0, v1);
+			q8_round(random, key, i, v0, vi, x0, y0);
+			q8_round(random, key, i + 1, v1, vi, x1, y1);
+			cm |= encode2<__NV_E4M3>(x0, x1) << (16 * j);
+			cv |= encode2<__NV_E5M2>(y0, y1) << (16 * j);
+		}
+		store_codes<WHOLE>(d.m, e + 128 * k, cm, left - 128 * k);
+		store_codes<WHOLE>(d.v, e + 128 * k, cv, left - 128 * k);
 	}
 }
 
+/* one tile: whole tiles, and runs of any length, on aligned addresses the fast way, other addresses element-wise */
 template <typename GradT, bool Q8>
-__device__ __forceinline__ void mt_update_phase(const mt_launch &a, const decision &dec, const q8_hyper &h)
+__device__ __forceinline__ void mt_tile(const mt_launch &a, const decision &dec, const mt_desc &d, void *grad,
+	uint32_t t, float (*slots)[2][ANNI_THREADS / 32], int &odd)
 {
-	const int64_t warp0 = (threadIdx.x >> 5) * ANNI_MT_BLOCK;
+	const bool vec = d.vec && ((uintptr_t)grad & 15) == 0 && !dec.skip;
+	const int64_t first = (int64_t)(t - d.tile0) * ANNI_MT_TILE;
+	const int64_t e0 = first + (threadIdx.x >> 5) * ANNI_MT_BLOCK;
+	const int64_t left = d.n - e0;
+	const int len = left < ANNI_MT_BLOCK ? (int)left : ANNI_MT_BLOCK;
 
-	/* backwards: the gradients read last by the norm phase are the likeliest to sit in L2 */
-	for (uint32_t r = (a.tiles + gridDim.x - 1) / gridDim.x; r > 0; r--) {
-		const uint32_t t = (r - 1) * gridDim.x + blockIdx.x;
+	if (vec && first + ANNI_MT_TILE <= d.n) {
+		if (Q8) {
+			run_vec_q8<GradT, true>(a, d, grad, e0, len, (float)dec.coef, slots[odd]);
+			odd ^= 1;
+		} else
+			run_vec_f32<GradT, true>(a, d, grad, e0, len, dec.coef);
+	} else if (left <= 0)
+		return;
+	else if (!vec)
+		run_scalar<GradT, Q8>(a, d, grad, e0, len, dec.coef, dec.skip);
+	else if (Q8)
+		run_vec_q8<GradT, false>(a, d, grad, e0, len, (float)dec.coef, NULL);
+	else
+		run_vec_f32<GradT, false>(a, d, grad, e0, len, dec.coef);
+}
 
-		if (t >= a.tiles)
-			continue;
-		const uint32_t s = a.tile_of[t];
-		void *grad = a.grad[s];
-		const mt_desc &d = a.desc[s];
-		const int64_t n = d.n;
-		const bool vec = d.vec && ((uintptr_t)grad & 15) == 0 && !dec.skip;
-		int64_t e0 = (int64_t)(t - d.tile0) * ANNI_MT_TILE + warp0;
+/* the entry of a tensor in shared memory */
+struct mt_held {
+	mt_desc	d;
+	void	*grad;
+};
 
-		if (!grad)
-			continue;
-#pragma unroll 1
-		for (int k = 0; k < ANNI_MT_TILE / ANNI_MT_PASS && e0 < n; k++, e0 += ANNI_MT_PASS) {
-			const int64_t left = n - e0;
+__device__ __forceinline__ void fetch(const mt_launch &a, uint32_t s, mt_held &to)
+{
+	const uint32_t i = threadIdx.x;
+	const uint32_t words = sizeof(mt_desc) / 4;
 
-			if (vec && left >= ANNI_MT_BLOCK) {
-				if (Q8)
-					run_vec_q8<GradT>(a, d, grad, e0, h);
-				else
-					run_vec_f32<GradT>(a, d, grad, e0, dec.coef);
-			} else
-				run_scalar<GradT, Q8>(a, d, grad, e0, left < ANNI_MT_BLOCK ? (int)left : ANNI_MT_BLOCK,
-				    dec.coef, h, dec.skip);
+	if (i < words + 2) {
+		const uint32_t *from = i < words ? reinterpret_cast<const uint32_t *>(a.desc + s) + i
+		    : reinterpret_cast<const uint32_t *>(a.grad + s) + (i - words);
+
+		asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" :: "r"((uint32_t)__cvta_generic_to_shared(
+		    reinterpret_cast<uint32_t *>(&to) + i)), "l"(from) : "memory");
+	}
+}
+
+__device__ __forceinline__ void fetched(void)
+{
+	asm volatile("cp.async.wait_all;" ::: "memory");
+	__syncthreads();
+}
+
+/*
+** Blocks take tiles round-robin, backwards: the whole grid works inside one small window of every buffer, and
+** the gradients read last by the norm phase are the likeliest to sit in L2.  A tile's tensor is looked up one
+** tile ahead, its entry is loaded into shared memory while the tile before is worked on.
+*/
+template <typename GradT, bool Q8>
+__device__ __forceinline__ void mt_update_phase(const mt_launch &a, const decision &dec)
+{
+	__shared__ float slots[2][2][ANNI_THREADS / 32];	/* new scales of m and v, two tiles */
+	__shared__ mt_held held[2];				/* this tile's tensor and the next one */
+	const uint32_t G = gridDim.x;
+	uint32_t r = (a.tiles + G - 1) / G;
+	uint32_t s;		/* tensor of this tile */
+	uint32_t next;		/* and of the next */
+	int cur = 0;
+	int odd = 0;
+
+	if (blockIdx.x >= a.tiles)
+		return;
+	if ((r - 1) * G + blockIdx.x >= a.tiles)
+		r--;
+	s = a.tile_of[(r - 1) * G + blockIdx.x];
+	next = r > 1 ? a.tile_of[(r - 2) * G + blockIdx.x] : s;
+	fetch(a, s, held[0]);
+	fetched();
+	for (; r > 0; r--) {
+		const uint32_t t = (r - 1) * G + blockIdx.x;
+		const bool change = next != s;
+
+		s = next;
+		if (r > 2)
+			next = a.tile_of[t - 2 * G];
+		if (change)
+			fetch(a, s, held[cur ^ 1]);	/* on its way while this tile is worked on */
+		if (held[cur].grad)
+			mt_tile<GradT, Q8>(a, dec, held[cur].d, held[cur].grad, t, slots, odd);
+		if (change) {
+			cur ^= 1;
+			fetched();
 		}
 	}
 }
@@ -416,20 +635,28 @@ __device__ __forceinline__ double mt_norm_phase(const mt_launch &a)
 		if (!grad)
 			continue;
 		if (((uintptr_t)grad & 15) == 0)
-			for (; i + 1024 <= len; i += 1024) {
+			for (; i + 256 <= len; i += 1024) {
 				f32x8 g[4];
 
 #pragma unroll
 				for (int k = 0; k < 4; k++)
-					g[k] = io8<GradT>::load_keep(grad, (uint64_t)lo + i + 256 * k + lane * 8);
+					if (i + 256 * k + 256 <= len)
+						g[k] = io8<GradT>::load_keep(grad, (uint64_t)lo + i + 256 * k + lane * 8);
 #pragma unroll
 				for (int k = 0; k < 4; k++)
-					norm_accumulate<GradT>(g[k], acc0, acc1);
+					if (i + 256 * k + 256 <= len)
+						norm_accumulate<GradT>(g[k], acc0, acc1);
 			}
-		for (i += lane; i < len; i += 32) {
-			const double g = (double)io8<GradT>::load1(grad, (uint64_t)lo + i);
+		/* what is left of the last 256, or everything on other alignments */
+		for (i = min(i, len & ~255); i < len; i += 256) {
+			float g[8];
 
-			acc0 = fma(g, g, acc0);
+#pragma unroll
+			for (int k = 0; k < 8; k++)
+				g[k] = i + 32 * k + lane < len ? io8<GradT>::load1(grad, (uint64_t)lo + i + 32 * k + lane) : 0.0f;
+#pragma unroll
+			for (int k = 0; k < 8; k++)
+				acc0 = fma((double)g[k], (double)g[k], acc0);
 		}
 	}
 	return acc0 + acc1;
@@ -439,7 +666,6 @@ template <typename GradT, bool Q8>
 __global__ void __launch_bounds__(ANNI_THREADS, 4) mt_step_kernel(const mt_launch a)
 {
 	decision d;
-	q8_hyper h;
 	double ss = 0.0;
 
 	if (a.la.flags & ANNI_LAUNCH_NEED_NORM) {
@@ -459,13 +685,8 @@ __global__ void __launch_bounds__(ANNI_THREADS, 4) mt_step_kernel(const mt_launc
 		a.la.ctl->eff_scale = d.coef;
 		a.la.ctl->skipped = d.skip ? 1 : 0;
 	}
-	h.b1 = (float)a.la.b1;
-	h.omb1 = (float)a.la.omb1;
-	h.b2 = (float)a.la.b2;
-	h.omb2 = (float)a.la.omb2;
-	h.coef = (float)d.coef;
 	if (!d.skip || (a.la.flags & ANNI_STEP_ZERO_GRAD))
-		mt_update_phase<GradT, Q8>(a, d, h);
+		mt_update_phase<GradT, Q8>(a, d);
 	step_epilogue(a.la.ctl, d.skip);
 }
 
@@ -757,6 +978,10 @@ extern "C" int anni_mtstep_step(anni_mtstep *h, const anni_optstep_hyper *hp, ui
 	a.tile_of = h->tile_of;
 	a.tiles = h->tiles;
 	a.seed = seed;
+	a.b1 = (float)a.la.b1;
+	a.omb1 = (float)a.la.omb1;
+	a.b2 = (float)a.la.b2;
+	a.omb2 = (float)a.la.omb2;
 	on_device dev(h->device);
 
 	if (!dev.ok)
