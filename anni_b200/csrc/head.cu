@@ -1,26 +1,49 @@
 /*
 ** Loss and gradients of a language model's head (include/anni_head.h).
 **
-** Forward: the logits of a tile of rows and vocabulary never leave the chip; each tile leaves the maximum and
-** the sum of exponentials of its rows, a small kernel joins the tiles of a row.  Backward: for one piece of the
-** vocabulary at a time, delta = softmax - one-hot is recomputed from lse and stored as bf16, then multiplied by
-** W^T into dx and by x^T into dw.
+** Four matrix products on the tensor cores, one persistent kernel each:
+**   loss    logits of a tile of rows and vocabulary; its epilogue keeps the maximum and the sum of exponentials
+**           of each row and drops the logits.  A small kernel joins the tiles of a row.
+**   delta   the same logits again for one piece of the vocabulary; softmax - one-hot from lse, stored as bf16
+**           (three terms of it for fp32 gradients), and its column sums for dbias
+**   dx      delta W^T of the piece, added to an fp32 sum over the pieces
+**   dw      x^T delta of the piece, stored or added to the gradient
+** Bound by the tensor cores: 2 T D V operations each (the logits twice, since they are not kept).
+**
+** A block (one per SM) works on 128 x 256 tiles: one thread loads tiles of both operands by TMA into a ring of
+** HEAD_STAGES stages, one thread issues tcgen05.mma into one of two accumulators in tensor memory, four warps
+** empty the other one.  An operand whose rows run along the summed dimension ("K-major") is loaded as one box
+** of 64 k x rows, one whose rows run along the result ("MN-major") as boxes of 64 mn x 64 k, so nothing is
+** transposed in memory.  Lengths that are no multiple of a tile end in zeros that TMA fills in.
 */
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
 #include <string.h>
 #include <algorithm>
+#include <mutex>
 #include "anni_head.h"
 #include "optstep_internal.h"
 
-#define HEAD_TM		64	/* rows and columns of a tile */
-#define HEAD_TN		64
+#define HEAD_TM		128	/* rows and columns of a tile */
+#define HEAD_TN		256
+#define HEAD_TK		64	/* 128 bytes of bf16: the widest swizzle */
+#define HEAD_STAGES	4
+#define HEAD_A_BYTES	(HEAD_TM * HEAD_TK * 2)
+#define HEAD_B_BYTES	(HEAD_TN * HEAD_TK * 2)
+#define HEAD_STAGE_BYTES (HEAD_A_BYTES + HEAD_B_BYTES)
+#define HEAD_MN_BYTES	(64 * HEAD_TK * 2)	/* one MN-major box */
+#define HEAD_THREADS	256
+#define HEAD_SMS	148	/* what the work is cut for; any number of SMs runs it */
 #define HEAD_PIECE_BYTES ((size_t)192 << 20)	/* of delta in the workspace */
 #define HEAD_TERMS	3	/* bf16 terms of delta for fp32 gradients */
+#define HEAD_WAIT_NS	2000000000ull	/* a wait inside a kernel gives up after this long */
 
 namespace {
+
+enum { LOSS, DELTA, DX, DW };
 
 struct head_args {
 	const __nv_bfloat16	*x;
@@ -39,12 +62,14 @@ struct head_args {
 	float			*hit;		/* logit of each row's target */
 	float2			*part;		/* [tiles over the vocabulary][tokens]: maximum, sum */
 	float			*row;		/* factor of each row, 0: no gradient */
-	__nv_bfloat16		*delta;		/* [terms][tokens][piece] */
+	__nv_bfloat16		*delta;		/* [terms][tokens][ldp] */
 	int			terms;
 	int64_t			ldp;
 	int			v0;		/* the piece: columns v0 .. v1 - 1 */
 	int			v1;
-	float			*dxp;		/* fp32 [tokens][d] */
+	float			*dxp;		/* fp32 [splits][tokens][ldd] */
+	int			ldd;
+	int			splits;
 	float			*dbp;		/* fp32 [row tiles][vocab] */
 	void			*dx;
 	int64_t			lddx;
@@ -56,28 +81,153 @@ struct head_args {
 	int			*error;
 };
 
-/* ---- one 64 x 64 tile of a product in fp32: 256 threads, 4 x 4 results each ----------------------- */
+struct gemm_args {
+	CUtensorMap	a;
+	CUtensorMap	b;
+	head_args	h;
+	int		m_tiles;
+	int		n_tiles;
+	int		k_blocks;	/* of one term */
+};
 
-template <typename A, typename B>
-__device__ __forceinline__ void tile_product(int k_end, A a, B b, float (&acc)[4][4])
+/* ---- PTX ------------------------------------------------------------------------------------------ */
+
+__device__ __forceinline__ uint32_t smem_of(const void *p)
 {
-	__shared__ float as[16][HEAD_TM + 4];
-	__shared__ float bs[16][HEAD_TN + 4];
-	const int tm = threadIdx.x / 16 * 4;
-	const int tn = threadIdx.x % 16 * 4;
+	return (uint32_t)__cvta_generic_to_shared(p);
+}
 
-	for (int k0 = 0; k0 < k_end; k0 += 16) {
-		for (int i = threadIdx.x; i < 16 * HEAD_TM; i += 256) {
-			as[i / HEAD_TM][i % HEAD_TM] = k0 + i / HEAD_TM < k_end ? a(i % HEAD_TM, k0 + i / HEAD_TM) : 0.0f;
-			bs[i / HEAD_TN][i % HEAD_TN] = k0 + i / HEAD_TN < k_end ? b(i % HEAD_TN, k0 + i / HEAD_TN) : 0.0f;
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count)
+{
+	asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(bar), "r"(count) : "memory");
+}
+
+__device__ __forceinline__ void mbar_arrive(uint32_t bar)
+{
+	asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes)
+{
+	asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(bar), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity)
+{
+	uint32_t ok;
+
+	asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+	    : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+	return ok != 0;
+}
+
+__device__ __forceinline__ uint64_t now_ns(void)
+{
+	uint64_t t;
+
+	asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+	return t;
+}
+
+/*
+** Waits for the barrier's phase of this parity.  Gives up, and says so to the whole block through `stop` and to
+** the host through `error`, after HEAD_WAIT_NS, or as soon as another thread of the block has given up
+** (stop NULL: only the time counts).
+*/
+__device__ __noinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity, volatile int *stop, int *error)
+{
+	const uint64_t end = now_ns() + HEAD_WAIT_NS;
+
+	for (;;) {
+		for (int k = 0; k < 64; k++)
+			if (mbar_try(bar, parity))
+				return true;
+		if (stop && *stop)
+			return false;
+		if (now_ns() > end) {
+			if (stop)
+				*stop = 1;
+			atomicExch(error, ANNI_E_BARRIER_TIMEOUT);
+			return false;
 		}
-		__syncthreads();
-		for (int k = 0; k < 16; k++)
-			for (int i = 0; i < 4; i++)
-				for (int j = 0; j < 4; j++)
-					acc[i][j] = fmaf(as[k][tm + i], bs[k][tn + j], acc[i][j]);
-		__syncthreads();
 	}
+}
+
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *stop, int *error)
+{
+	return mbar_try(bar, parity) || mbar_wait_long(bar, parity, stop, error);
+}
+
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1, int c2)
+{
+	asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+	    :: "r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
+}
+
+/*
+** Shared-memory descriptor of an operand tile with 128-byte swizzle (all distances in units of 16 bytes).
+** K-major: rows of 128 bytes, eight rows to a swizzle atom, atoms 1024 bytes apart (the stride field); the
+** leading field is not used.  MN-major: boxes of 64 mn x 64 k; eight k to an atom, atoms 1024 bytes apart
+** (the stride field), the next 64 mn one box further (the leading field).
+*/
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, bool mn)
+{
+	const uint64_t lead = mn ? HEAD_MN_BYTES >> 4 : 1;
+
+	return (uint64_t)((addr & 0x3ffff) >> 4) | lead << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+/* D (fp32) = A B, both bf16: M 128, N 256, and which of them are MN-major */
+__device__ __forceinline__ constexpr uint32_t instr_desc(bool a_mn, bool b_mn)
+{
+	return 1u << 4 | 1u << 7 | 1u << 10 | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | (uint32_t)(HEAD_TN >> 3) << 17
+	    | (uint32_t)(HEAD_TM >> 4) << 24;
+}
+
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add)
+{
+	asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+	    "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+	    :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+}
+
+__device__ __forceinline__ void mma_commit(uint32_t bar)
+{
+	asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory");
+}
+
+/* 32 columns of this warp's 32 lanes of tensor memory: lane l gets row l */
+__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32])
+{
+	uint32_t r[32];
+
+	__syncwarp();		/* rows that do not exist go other ways between two loads */
+	asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+	    "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+	    "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+	    : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+	    "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+	    "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+	    "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]) : "r"(addr));
+	asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+	for (int i = 0; i < 32; i++)
+		v[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ float exp2_approx(float x)
+{
+	float r;
+
+	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+	return r;
+}
+
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi)
+{
+	const __nv_bfloat162 q = __floats2bfloat162_rn(lo, hi);
+
+	return *reinterpret_cast<const uint32_t *>(&q);
 }
 
 __device__ __forceinline__ float to_f(__nv_bfloat16 v)
@@ -85,139 +235,265 @@ __device__ __forceinline__ float to_f(__nv_bfloat16 v)
 	return __bfloat162float(v);
 }
 
-/* logits of the tile at (t0, v0), bias included; -inf beyond the vocabulary */
-__device__ __forceinline__ void logits_tile(const head_args &h, int t0, int v0, float (*out)[HEAD_TN + 1])
+#define LOG2E	1.44269504088896340736f
+
+/* ---- which tile, and what of it a stage holds ---------------------------------------------------- */
+
+struct tile_at {
+	int	m0;
+	int	n0;
+	int	k0;	/* k blocks lo .. hi - 1 of each term */
+	int	k1;
+	int	split;
+};
+
+/*
+** Order of the tiles.  loss, delta: all row tiles (64 at most) of one column tile after another, so that W is
+** read once while x stays in L2; dx: the column tiles of a row tile together, dw: the row tiles of a column tile
+** together, so that delta is read once.
+*/
+template <int KIND>
+__device__ __forceinline__ tile_at tile_of(const gemm_args &g, int t)
 {
-	float acc[4][4] = {};
-	const int tm = threadIdx.x / 16 * 4;
-	const int tn = threadIdx.x % 16 * 4;
+	tile_at r;
+	int m;
+	int n;
 
-	tile_product(h.d, [&](int m, int k) { return t0 + m < h.tokens ? to_f(h.x[(int64_t)(t0 + m) * h.ldx + k]) : 0.0f; },
-	    [&](int n, int k) { return v0 + n < h.vocab ? to_f(h.w[(int64_t)k * h.ldw + v0 + n]) : 0.0f; }, acc);
-	for (int i = 0; i < 4; i++)
-		for (int j = 0; j < 4; j++) {
-			const int v = v0 + tn + j;
+	r.split = 0;
+	r.k0 = 0;
+	r.k1 = g.k_blocks;
+	if (KIND == DX) {
+		n = t % g.n_tiles;
+		m = t / g.n_tiles % g.m_tiles;
+		r.split = t / (g.n_tiles * g.m_tiles);
+		r.k0 = (int)((int64_t)g.k_blocks * r.split / g.h.splits);
+		r.k1 = (int)((int64_t)g.k_blocks * (r.split + 1) / g.h.splits);
+	} else if (KIND == DW) {
+		m = t % g.m_tiles;
+		n = t / g.m_tiles;
+	} else {
+		const int group = t / (64 * g.n_tiles);
+		const int rows = min(64, g.m_tiles - group * 64);
+		const int i = t - group * 64 * g.n_tiles;
 
-			out[tm + i][tn + j] = v >= h.vocab ? -INFINITY : acc[i][j] + (h.bias ? h.bias[v] : 0.0f);
-		}
-	__syncthreads();
+		m = group * 64 + i % rows;
+		n = i / rows;
+	}
+	r.m0 = m * HEAD_TM;
+	r.n0 = n * HEAD_TN;
+	return r;
 }
 
-__global__ void __launch_bounds__(256) loss_kernel(const head_args h)
+template <int KIND>
+__device__ __forceinline__ void load_stage(const gemm_args &g, const tile_at &t, int term, int k, uint32_t dst, uint32_t bar)
 {
-	__shared__ float z[HEAD_TM][HEAD_TN + 1];
-	const int t0 = blockIdx.y * HEAD_TM;
-	const int v0 = blockIdx.x * HEAD_TN;
-	const int t = t0 + threadIdx.x;
+	const uint32_t b = dst + HEAD_A_BYTES;
 
-	logits_tile(h, t0, v0, z);
-	if (threadIdx.x < HEAD_TM && t < h.tokens) {
-		float top = -INFINITY;
-		float sum = 0.0f;
-		const int y = h.target[t];
-
-		for (int j = 0; j < HEAD_TN; j++)
-			top = fmaxf(top, z[threadIdx.x][j]);
-		for (int j = 0; j < HEAD_TN; j++)
-			sum += expf(z[threadIdx.x][j] - (top == -INFINITY ? 0.0f : top));
-		h.part[(int64_t)blockIdx.x * h.tokens + t] = make_float2(top, sum);
-		if (y >= v0 && y < v0 + HEAD_TN && y < h.vocab)
-			h.hit[t] = z[threadIdx.x][y - v0];
+	if (KIND == LOSS || KIND == DELTA) {
+		tma_load(dst, &g.a, bar, k, t.m0, 0);
+#pragma unroll
+		for (int j = 0; j < HEAD_TN / 64; j++)
+			tma_load(b + j * HEAD_MN_BYTES, &g.b, bar, g.h.v0 + t.n0 + 64 * j, k, 0);
+	} else if (KIND == DX) {
+		tma_load(dst, &g.a, bar, k, t.m0, term);
+		tma_load(b, &g.b, bar, g.h.v0 + k, t.n0, 0);
+	} else {
+#pragma unroll
+		for (int j = 0; j < HEAD_TM / 64; j++)
+			tma_load(dst + j * HEAD_MN_BYTES, &g.a, bar, t.m0 + 64 * j, k, 0);
+#pragma unroll
+		for (int j = 0; j < HEAD_TN / 64; j++)
+			tma_load(b + j * HEAD_MN_BYTES, &g.b, bar, t.n0 + 64 * j, k, term);
 	}
 }
 
-__global__ void __launch_bounds__(256) join_kernel(const head_args h, int tiles)
+/* ---- epilogues: one warp's 32 rows of a tile, 32 columns at a time -------------------------------- */
+
+struct epi_smem {
+	float	bias[2][HEAD_TN];	/* of two tiles; -inf beyond the vocabulary */
+	float	sums[2][4][HEAD_TN];	/* delta: column sums of each warp's rows */
+};
+
+__device__ __forceinline__ void epi_barrier(void)
 {
-	const int t = blockIdx.x * blockDim.x + threadIdx.x;
+	asm volatile("bar.sync 1, 128;" ::: "memory");
+}
+
+/* biases of the tile's columns, staged by the four epilogue warps */
+__device__ __forceinline__ void stage_bias(const head_args &h, int v0, int end, float *to)
+{
+	for (int i = threadIdx.x & 127; i < HEAD_TN; i += 128)
+		to[i] = v0 + i >= end ? -INFINITY : h.bias ? __ldg(h.bias + v0 + i) : 0.0f;
+	epi_barrier();
+}
+
+/* v[i] + sum over the warp's rows: lane l ends with the sum of column l, rows added in a fixed tree */
+__device__ __forceinline__ float column_sums(float (&v)[32])
+{
+	const int lane = threadIdx.x & 31;
+
+#pragma unroll
+	for (int s = 16; s > 0; s >>= 1) {
+		const bool up = lane & s;
+
+#pragma unroll
+		for (int i = 0; i < s; i++) {
+			const float send = up ? v[i] : v[i + s];
+			const float keep = up ? v[i + s] : v[i];
+
+			v[i] = keep + __shfl_xor_sync(0xffffffffu, send, s);
+		}
+	}
+	return v[0];
+}
+
+/* one pass over the columns with a running maximum and a sum that follows it */
+__device__ __forceinline__ void loss_epilogue(const gemm_args &g, const tile_at &at, uint32_t tmem, const float *bias)
+{
+	const head_args &h = g.h;
+	const int t = at.m0 + (threadIdx.x & 127);
+	const int y = t < h.tokens ? h.target[t] : -1;
+	const int rel = y >= at.n0 && y < h.vocab && y < at.n0 + HEAD_TN ? y - at.n0 : -1;
 	float top = -INFINITY;
 	float sum = 0.0f;
-	float lse;
-	int y;
 
-	if (t >= h.tokens)
-		return;
-	for (int k = 0; k < tiles; k++)
-		top = fmaxf(top, h.part[(int64_t)k * h.tokens + t].x);
-	for (int k = 0; k < tiles; k++) {
-		const float2 p = h.part[(int64_t)k * h.tokens + t];
+#pragma unroll 1
+	for (int c = 0; c < HEAD_TN; c += 32) {
+		float v[32];
+		float high;
+		float base;
 
-		if (p.x != -INFINITY)
-			sum += p.y * expf(p.x - top);
+		tmem_load(tmem + c, v);
+#pragma unroll
+		for (int i = 0; i < 32; i += 4) {
+			const float4 b = *reinterpret_cast<const float4 *>(bias + c + i);
+
+			v[i] += b.x;
+			v[i + 1] += b.y;
+			v[i + 2] += b.z;
+			v[i + 3] += b.w;
+		}
+		if (__any_sync(0xffffffffu, rel >= c && rel < c + 32)) {	/* one in vocab / 32 chunks of a row */
+#pragma unroll
+			for (int i = 0; i < 32; i++)
+				if (rel == c + i)
+					h.hit[t] = v[i];
+		}
+		high = v[0];
+#pragma unroll
+		for (int i = 1; i < 32; i++)
+			high = fmaxf(high, v[i]);
+		high = fmaxf(high, top);
+		base = high == -INFINITY ? 0.0f : high;
+		sum *= exp2_approx((top - base) * LOG2E);
+		top = high;
+#pragma unroll
+		for (int i = 0; i < 32; i++)
+			sum += exp2_approx((v[i] - base) * LOG2E);
 	}
-	lse = top + logf(sum);
-	y = h.target[t];
-	h.lse[t] = lse;
-	h.nll[t] = y < 0 ? 0.0f : y >= h.vocab ? NAN : lse - h.hit[t];
+	if (t < h.tokens)
+		h.part[(int64_t)(at.n0 / HEAD_TN) * h.tokens + t] = make_float2(top, sum);
 }
 
-__global__ void __launch_bounds__(256) row_kernel(const head_args h)
+__device__ __forceinline__ void delta_epilogue(const gemm_args &g, const tile_at &at, uint32_t tmem, const float *bias,
+	float (*sums)[HEAD_TN])
 {
-	const int t = blockIdx.x * blockDim.x + threadIdx.x;
+	const head_args &h = g.h;
+	const int lane = threadIdx.x & 31;
+	const int wq = threadIdx.x >> 5 & 3;
+	const int t = at.m0 + (threadIdx.x & 127);
+	const float f = t < h.tokens ? h.row[t] : 0.0f;
+	const float lse = f != 0.0f ? h.lse[t] : 0.0f;
+	const int y = f != 0.0f ? h.target[t] - h.v0 - at.n0 : -1;
+	__nv_bfloat16 *out = h.delta + (int64_t)t * h.ldp + at.n0;
 
-	if (t < h.tokens) {
-		const bool on = h.target[t] >= 0 && h.target[t] < h.vocab && h.lse[t] != -INFINITY;
+#pragma unroll 1
+	for (int c = 0; c < HEAD_TN; c += 32) {
+		float v[32];
 
-		h.row[t] = on ? h.scale * (h.weight ? h.weight[t] : 1.0f) : 0.0f;
-	}
-}
+		tmem_load(tmem + c, v);
+#pragma unroll
+		for (int i = 0; i < 32; i += 4) {
+			const float4 b = *reinterpret_cast<const float4 *>(bias + c + i);
 
-__global__ void __launch_bounds__(256) delta_kernel(const head_args h)
-{
-	__shared__ float z[HEAD_TM][HEAD_TN + 1];
-	const int t0 = blockIdx.y * HEAD_TM;
-	const int v0 = h.v0 + blockIdx.x * HEAD_TN;
+			v[i] = exp2_approx((v[i] + b.x - lse) * LOG2E);
+			v[i + 1] = exp2_approx((v[i + 1] + b.y - lse) * LOG2E);
+			v[i + 2] = exp2_approx((v[i + 2] + b.z - lse) * LOG2E);
+			v[i + 3] = exp2_approx((v[i + 3] + b.w - lse) * LOG2E);
+		}
+		if (__any_sync(0xffffffffu, y >= c && y < c + 32)) {
+#pragma unroll
+			for (int i = 0; i < 32; i++)
+				if (y == c + i)
+					v[i] -= 1.0f;
+		}
+#pragma unroll
+		for (int i = 0; i < 32; i++)
+			v[i] = f != 0.0f ? v[i] * f : 0.0f;
+		if (t < h.tokens) {
+			float rest[32];
 
-	logits_tile(h, t0, v0, z);
-	for (int i = threadIdx.x; i < HEAD_TM * HEAD_TN; i += 256) {
-		const int t = t0 + i / HEAD_TN;
-		const int v = v0 + i % HEAD_TN;
-		float dl = 0.0f;
-
-		if (t < h.tokens && v < h.v1 && h.row[t] != 0.0f) {
-			float rest;
-
-			dl = h.row[t] * (expf(z[i / HEAD_TN][i % HEAD_TN] - h.lse[t]) - (v == h.target[t] ? 1.0f : 0.0f));
-			rest = dl;
+#pragma unroll
+			for (int i = 0; i < 32; i++)
+				rest[i] = v[i];
+			/* the largest term last: the products add the small ones up first */
 			for (int k = h.terms - 1; k >= 0; k--) {
-				const __nv_bfloat16 q = __float2bfloat16_rn(rest);
+				uint4 *q = reinterpret_cast<uint4 *>(out + (int64_t)k * h.tokens * h.ldp + c);
 
-				h.delta[((int64_t)k * h.tokens + t) * h.ldp + v - h.v0] = q;
-				rest -= to_f(q);
+#pragma unroll
+				for (int i = 0; i < 32; i += 8) {
+					uint4 r;
+
+					r.x = bf16_pair(rest[i], rest[i + 1]);
+					r.y = bf16_pair(rest[i + 2], rest[i + 3]);
+					r.z = bf16_pair(rest[i + 4], rest[i + 5]);
+					r.w = bf16_pair(rest[i + 6], rest[i + 7]);
+					q[i / 8] = r;
+				}
+				if (k > 0)
+#pragma unroll
+					for (int i = 0; i < 32; i++)
+						rest[i] -= to_f(__float2bfloat16_rn(rest[i]));
 			}
-		} else if (t < h.tokens && v < h.v1)
-			for (int k = 0; k < h.terms; k++)
-				h.delta[((int64_t)k * h.tokens + t) * h.ldp + v - h.v0] = __float2bfloat16_rn(0.0f);
-		z[i / HEAD_TN][i % HEAD_TN] = dl;
+		}
+		if (h.db)
+			sums[wq][c + lane] = column_sums(v);
 	}
-	__syncthreads();
-	if (threadIdx.x < HEAD_TN && v0 + (int)threadIdx.x < h.v1) {
-		float s = 0.0f;
-
-		for (int k = 0; k < HEAD_TM; k++)
-			s += z[k][threadIdx.x];
-		h.dbp[(int64_t)blockIdx.y * h.vocab + v0 + threadIdx.x] = s;
+	if (h.db) {
+		epi_barrier();
+		for (int i = threadIdx.x & 127; i < HEAD_TN; i += 128)
+			if (h.v0 + at.n0 + i < h.v1)
+				h.dbp[(int64_t)(at.m0 / HEAD_TM) * h.vocab + h.v0 + at.n0 + i] =
+				    (sums[0][i] + sums[1][i]) + (sums[2][i] + sums[3][i]);
 	}
 }
 
-__global__ void __launch_bounds__(256) dx_kernel(const head_args h)
+__device__ __forceinline__ void dx_epilogue(const gemm_args &g, const tile_at &at, uint32_t tmem)
 {
-	float acc[4][4] = {};
-	const int t0 = blockIdx.y * HEAD_TM;
-	const int d0 = blockIdx.x * HEAD_TN;
-	const int tm = threadIdx.x / 16 * 4;
-	const int tn = threadIdx.x % 16 * 4;
+	const head_args &h = g.h;
+	const int t = at.m0 + (threadIdx.x & 127);
+	float *out = h.dxp + ((int64_t)at.split * h.tokens + t) * h.ldd + at.n0;
 
-	for (int p = 0; p < h.terms; p++)
-		tile_product(h.v1 - h.v0, [&](int m, int k) { return t0 + m < h.tokens
-		    ? to_f(h.delta[((int64_t)p * h.tokens + t0 + m) * h.ldp + k]) : 0.0f; },
-		    [&](int n, int k) { return d0 + n < h.d ? to_f(h.w[(int64_t)(d0 + n) * h.ldw + h.v0 + k]) : 0.0f; }, acc);
-	for (int i = 0; i < 4; i++)
-		for (int j = 0; j < 4; j++)
-			if (t0 + tm + i < h.tokens && d0 + tn + j < h.d) {
-				float *q = &h.dxp[(int64_t)(t0 + tm + i) * h.d + d0 + tn + j];
+#pragma unroll 1
+	for (int c = 0; c < HEAD_TN && at.n0 + c < h.ldd; c += 32) {
+		float v[32];
 
-				*q = (h.v0 ? *q : 0.0f) + acc[i][j];
+		tmem_load(tmem + c, v);
+		if (t >= h.tokens)
+			continue;
+#pragma unroll
+		for (int i = 0; i < 32; i += 4)
+			if (at.n0 + c + i < h.ldd) {
+				float4 *q = reinterpret_cast<float4 *>(out + c + i);
+				float4 r = h.v0 ? *q : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+
+				r.x += v[i];
+				r.y += v[i + 1];
+				r.z += v[i + 2];
+				r.w += v[i + 3];
+				*q = r;
 			}
+	}
 }
 
 __device__ __forceinline__ void put(void *base, int64_t i, float v, int bf16, int add)
@@ -233,30 +509,320 @@ __device__ __forceinline__ void put(void *base, int64_t i, float v, int bf16, in
 	}
 }
 
-__global__ void __launch_bounds__(256) dw_kernel(const head_args h)
+__device__ __forceinline__ float2 unpack2(uint32_t q)
 {
-	float acc[4][4] = {};
-	const int d0 = blockIdx.y * HEAD_TM;
-	const int v0 = h.v0 + blockIdx.x * HEAD_TN;
-	const int tm = threadIdx.x / 16 * 4;
-	const int tn = threadIdx.x % 16 * 4;
+	return make_float2(__uint_as_float(q << 16), __uint_as_float(q & 0xffff0000u));
+}
 
-	for (int p = 0; p < h.terms; p++)
-		tile_product(h.tokens, [&](int m, int k) { return d0 + m < h.d && h.row[k] != 0.0f
-		    ? to_f(h.x[(int64_t)k * h.ldx + d0 + m]) : 0.0f; },
-		    [&](int n, int k) { return v0 + n < h.v1
-		    ? to_f(h.delta[((int64_t)p * h.tokens + k) * h.ldp + v0 - h.v0 + n]) : 0.0f; }, acc);
-	for (int i = 0; i < 4; i++)
-		for (int j = 0; j < 4; j++)
-			if (d0 + tm + i < h.d && v0 + tn + j < h.v1)
-				put(h.dw, (int64_t)(d0 + tm + i) * h.lddw + v0 + tn + j, acc[i][j], h.bf16, h.add);
+__device__ __forceinline__ void dw_epilogue(const gemm_args &g, const tile_at &at, uint32_t tmem)
+{
+	const head_args &h = g.h;
+	const int d = at.m0 + (threadIdx.x & 127);
+	const int v0 = h.v0 + at.n0;
+	const int size = h.bf16 ? 2 : 4;
+	const int64_t first = (int64_t)d * h.lddw + v0;
+	char *out = static_cast<char *>(h.dw) + first * size;
+	const bool vec = ((uintptr_t)out & 15) == 0;
+
+#pragma unroll 1
+	for (int c = 0; c < HEAD_TN && v0 + c < h.v1; c += 32) {
+		float v[32];
+
+		tmem_load(tmem + c, v);
+		if (d >= h.d)
+			continue;
+		if (!vec || v0 + c + 32 > h.v1) {
+#pragma unroll
+			for (int i = 0; i < 32; i++)
+				if (v0 + c + i < h.v1)
+					put(h.dw, first + c + i, v[i], h.bf16, h.add);
+		} else if (h.bf16) {
+			uint4 *q = reinterpret_cast<uint4 *>(out + c * 2);
+
+#pragma unroll
+			for (int i = 0; i < 32; i += 8) {
+				uint4 r = h.add ? q[i / 8] : make_uint4(0, 0, 0, 0);
+				const float2 r0 = unpack2(r.x);
+				const float2 r1 = unpack2(r.y);
+				const float2 r2 = unpack2(r.z);
+				const float2 r3 = unpack2(r.w);
+
+				r.x = bf16_pair(r0.x + v[i], r0.y + v[i + 1]);
+				r.y = bf16_pair(r1.x + v[i + 2], r1.y + v[i + 3]);
+				r.z = bf16_pair(r2.x + v[i + 4], r2.y + v[i + 5]);
+				r.w = bf16_pair(r3.x + v[i + 6], r3.y + v[i + 7]);
+				q[i / 8] = r;
+			}
+		} else {
+			float4 *q = reinterpret_cast<float4 *>(out + c * 4);
+
+#pragma unroll
+			for (int i = 0; i < 32; i += 4) {
+				float4 r = h.add ? q[i / 4] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+
+				r.x += v[i];
+				r.y += v[i + 1];
+				r.z += v[i + 2];
+				r.w += v[i + 3];
+				q[i / 4] = r;
+			}
+		}
+	}
+}
+
+/* ---- the product -------------------------------------------------------------------------------------- */
+
+struct gemm_smem {
+	uint64_t	full[HEAD_STAGES];	/* a stage has been loaded */
+	uint64_t	empty[HEAD_STAGES];	/* ... and consumed */
+	uint64_t	ready[2];		/* an accumulator is complete */
+	uint64_t	drained[2];		/* ... and read out */
+	uint64_t	quiet;			/* after a give-up: the products in flight are done */
+	uint32_t	tmem;
+	int		stop;			/* somebody has given up */
+	epi_smem	epi;
+};
+
+/* loads; returns after a give-up only when its own copies have landed (or the time is up) */
+template <int KIND>
+__device__ __forceinline__ void producer(const gemm_args &g, gemm_smem *s, uint32_t ring, int total)
+{
+	uint32_t n = 0;		/* stages loaded so far */
+
+	for (int tile = blockIdx.x; tile < total; tile += gridDim.x) {
+		const tile_at at = tile_of<KIND>(g, tile);
+
+		for (int term = 0; term < (KIND == DX || KIND == DW ? g.h.terms : 1); term++)
+			for (int k = at.k0; k < at.k1; k++, n++) {
+				const uint32_t i = n % HEAD_STAGES;
+
+				if (!mbar_wait(smem_of(&s->empty[i]), (n / HEAD_STAGES & 1) ^ 1, &s->stop, g.h.error)) {
+					for (uint32_t j = n < HEAD_STAGES ? 0 : n - HEAD_STAGES; j < n; j++)
+						(void)mbar_wait(smem_of(&s->full[j % HEAD_STAGES]), j / HEAD_STAGES & 1, NULL,
+						    g.h.error);
+					return;
+				}
+				mbar_expect(smem_of(&s->full[i]), HEAD_STAGE_BYTES);
+				load_stage<KIND>(g, at, KIND == DX || KIND == DW ? g.h.terms - 1 - term : 0, k * HEAD_TK,
+				    ring + i * HEAD_STAGE_BYTES, smem_of(&s->full[i]));
+			}
+	}
+}
+
+template <int KIND>
+__device__ __forceinline__ void multiplier(const gemm_args &g, gemm_smem *s, uint32_t ring, int total)
+{
+	const bool a_mn = KIND == DW;
+	const bool b_mn = KIND != DX;
+	const uint32_t idesc = instr_desc(a_mn, b_mn);
+	uint32_t n = 0;
+	uint32_t done = 0;	/* tiles */
+
+	for (int tile = blockIdx.x; tile < total; tile += gridDim.x, done++) {
+		const tile_at at = tile_of<KIND>(g, tile);
+		const int steps = (at.k1 - at.k0) * (KIND == DX || KIND == DW ? g.h.terms : 1);
+		const uint32_t acc = s->tmem + (done & 1) * HEAD_TN;
+		bool ok = mbar_wait(smem_of(&s->drained[done & 1]), (done / 2 & 1) ^ 1, &s->stop, g.h.error);
+
+		asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+		for (int k = 0; ok && k < steps; k++, n++) {
+			const uint32_t i = n % HEAD_STAGES;
+			const uint32_t base = ring + i * HEAD_STAGE_BYTES;
+
+			ok = mbar_wait(smem_of(&s->full[i]), n / HEAD_STAGES & 1, &s->stop, g.h.error);
+			if (!ok)
+				break;
+			asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+			/* 16 k a time: 32 bytes further in a K-major row, 16 rows of 128 bytes further in an MN-major box */
+#pragma unroll
+			for (int j = 0; j < HEAD_TK / 16; j++)
+				mma(acc, smem_desc(base + j * (a_mn ? 2048 : 32), a_mn),
+				    smem_desc(base + HEAD_A_BYTES + j * (b_mn ? 2048 : 32), b_mn), idesc, k > 0 || j > 0);
+			mma_commit(smem_of(&s->empty[i]));
+		}
+		if (!ok) {
+			mma_commit(smem_of(&s->quiet));
+			(void)mbar_wait(smem_of(&s->quiet), 0, NULL, g.h.error);
+			return;
+		}
+		mma_commit(smem_of(&s->ready[done & 1]));
+	}
+}
+
+template <int KIND>
+__device__ __forceinline__ void drainer(const gemm_args &g, gemm_smem *s, int total)
+{
+	const uint32_t lanes = (uint32_t)(threadIdx.x >> 5 & 3) << 21;	/* this warp's quarter of the lanes: 32 w << 16 */
+	uint32_t done = 0;
+
+	for (int tile = blockIdx.x; tile < total; tile += gridDim.x, done++) {
+		const tile_at at = tile_of<KIND>(g, tile);
+		const uint32_t b = done & 1;
+		const uint32_t acc = s->tmem + lanes + b * HEAD_TN;
+
+		if (KIND == LOSS)
+			stage_bias(g.h, at.n0, g.h.vocab, s->epi.bias[b]);
+		if (KIND == DELTA)
+			stage_bias(g.h, g.h.v0 + at.n0, g.h.v1, s->epi.bias[b]);
+		/* the whole warp waits; it keeps step with the other warps even after a give-up, for the barriers' sake */
+		(void)mbar_wait(smem_of(&s->ready[b]), done / 2 & 1, &s->stop, g.h.error);
+		__syncwarp();
+		asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+		if (KIND == LOSS)
+			loss_epilogue(g, at, acc, s->epi.bias[b]);
+		else if (KIND == DELTA)
+			delta_epilogue(g, at, acc, s->epi.bias[b], s->epi.sums[b]);
+		else if (KIND == DX)
+			dx_epilogue(g, at, acc);
+		else
+			dw_epilogue(g, at, acc);
+		asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+		__syncwarp();
+		if ((threadIdx.x & 31) == 0)
+			mbar_arrive(smem_of(&s->drained[b]));
+	}
+}
+
+template <int KIND>
+__global__ void __launch_bounds__(HEAD_THREADS, 1) product_kernel(const __grid_constant__ gemm_args g)
+{
+	extern __shared__ uint8_t dynamic[];
+	__shared__ gemm_smem s;
+	const uint32_t ring = (smem_of(dynamic) + 1023) & ~1023u;	/* swizzle atoms lie on 1024 bytes */
+	const int warp = threadIdx.x >> 5;
+	const int total = g.m_tiles * g.n_tiles * (KIND == DX ? g.h.splits : 1);
+
+	if (threadIdx.x == 0) {
+		for (int i = 0; i < HEAD_STAGES; i++) {
+			mbar_init(smem_of(&s.full[i]), 1);
+			mbar_init(smem_of(&s.empty[i]), 1);
+		}
+		for (int i = 0; i < 2; i++) {
+			mbar_init(smem_of(&s.ready[i]), 1);
+			mbar_init(smem_of(&s.drained[i]), 4);
+		}
+		mbar_init(smem_of(&s.quiet), 1);
+		s.stop = 0;
+		asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+		asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+	}
+	if (warp == 2) {
+		asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" :: "r"(smem_of(&s.tmem)) : "memory");
+		asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+	}
+	asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+	__syncthreads();
+	asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+	if (warp == 0) {
+		if ((threadIdx.x & 31) == 0)
+			producer<KIND>(g, &s, ring, total);
+		__syncwarp();
+	} else if (warp == 1) {
+		if ((threadIdx.x & 31) == 0)
+			multiplier<KIND>(g, &s, ring, total);
+		__syncwarp();
+	} else if (warp >= 4)
+		drainer<KIND>(g, &s, total);
+	asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+	__syncthreads();
+	asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+	if (warp == 2)
+		asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" :: "r"(s.tmem) : "memory");
+}
+
+/* ---- what goes before and after the products ------------------------------------------------------------ */
+
+/* joins the tiles of a row: eight warps share the tiles of 32 rows */
+__global__ void __launch_bounds__(256) join_kernel(const head_args h, int tiles)
+{
+	__shared__ float2 s[8][32];
+	const int t = blockIdx.x * 32 + (threadIdx.x & 31);
+	const int w = threadIdx.x >> 5;
+	float top = -INFINITY;
+	float sum = 0.0f;
+	float lse;
+	int y;
+
+	if (t < h.tokens)
+		for (int k = w; k < tiles; k += 8) {
+			const float2 p = h.part[(int64_t)k * h.tokens + t];
+			const float high = fmaxf(top, p.x);
+			const float base = high == -INFINITY ? 0.0f : high;
+
+			sum = sum * exp2f((top - base) * LOG2E) + p.y * exp2f((p.x - base) * LOG2E);
+			top = high;
+		}
+	s[w][threadIdx.x & 31] = make_float2(top, sum);
+	__syncthreads();
+	if (w != 0 || t >= h.tokens)
+		return;
+	for (int k = 1; k < 8; k++) {
+		const float2 p = s[k][threadIdx.x];
+		const float high = fmaxf(top, p.x);
+		const float base = high == -INFINITY ? 0.0f : high;
+
+		sum = sum * exp2f((top - base) * LOG2E) + p.y * exp2f((p.x - base) * LOG2E);
+		top = high;
+	}
+	lse = *h.error ? NAN : top + logf(sum);
+	y = h.target[t];
+	h.lse[t] = lse;
+	h.nll[t] = y < 0 ? (*h.error ? NAN : 0.0f) : y >= h.vocab ? NAN : lse - h.hit[t];
+}
+
+/* factor of each row: 0 where there is no gradient */
+__device__ __forceinline__ float row_factor(const head_args &h, int t)
+{
+	const int y = h.target[t];
+
+	return y >= 0 && y < h.vocab && h.lse[t] != -INFINITY ? h.scale * (h.weight ? h.weight[t] : 1.0f) : 0.0f;
+}
+
+/*
+** Rows of bf16 to a 16-byte grid, one block per row.  With ROWS also their factors, and zeros for the rows
+** without a gradient, so that whatever they hold meets a delta of 0 as 0.
+*/
+template <bool ROWS>
+__global__ void __launch_bounds__(128) pack_kernel(const head_args h, __nv_bfloat16 *to, int64_t ldt, const __nv_bfloat16 *from,
+	int64_t ldf, int rows, int cols)
+{
+	for (int r = blockIdx.x; r < rows; r += gridDim.x) {
+		const float f = ROWS ? row_factor(h, r) : 1.0f;
+		const __nv_bfloat16 *src = from + (int64_t)r * ldf;
+		__nv_bfloat16 *dst = to + (int64_t)r * ldt;
+		const bool on = f != 0.0f;
+
+		if (ROWS && threadIdx.x == 0)
+			h.row[r] = f;
+		if (((uintptr_t)src & 15) == 0)
+			for (int i = threadIdx.x * 8; i < cols; i += 128 * 8) {
+				if (i + 8 <= cols)
+					*reinterpret_cast<uint4 *>(dst + i) = on ? *reinterpret_cast<const uint4 *>(src + i)
+					    : make_uint4(0, 0, 0, 0);
+				else
+					for (int j = i; j < cols; j++)
+						dst[j] = on ? src[j] : __float2bfloat16_rn(0.0f);
+			}
+		else
+			for (int i = threadIdx.x; i < cols; i += 128)
+				dst[i] = on ? src[i] : __float2bfloat16_rn(0.0f);
+	}
 }
 
 __global__ void __launch_bounds__(256) finish_dx_kernel(const head_args h)
 {
+	const bool bad = *h.error != 0;
+
 	for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < (int64_t)h.tokens * h.d;
-	    i += (int64_t)gridDim.x * blockDim.x)
-		put(h.dx, i / h.d * h.lddx + i % h.d, h.dxp[i], h.bf16, 0);
+	    i += (int64_t)gridDim.x * blockDim.x) {
+		const int64_t t = i / h.d;
+		const int64_t d = i - t * h.d;
+		float v = 0.0f;
+
+		for (int k = 0; k < h.splits; k++)
+			v += h.dxp[((int64_t)k * h.tokens + t) * h.ldd + d];
+		put(h.dx, t * h.lddx + d, bad ? NAN : v, h.bf16, 0);
+	}
 }
 
 __global__ void __launch_bounds__(256) finish_db_kernel(const head_args h, int tiles)
@@ -268,8 +834,9 @@ __global__ void __launch_bounds__(256) finish_db_kernel(const head_args h, int t
 		return;
 	for (int k = 0; k < tiles; k++)
 		s += (double)h.dbp[(int64_t)k * h.vocab + v];
-	put(h.db, v, (float)(s + (h.add ? h.bf16 ? (double)to_f(static_cast<__nv_bfloat16 *>(h.db)[v])
-	    : (double)static_cast<float *>(h.db)[v] : 0.0)), h.bf16, 0);
+	if (h.add)
+		s += h.bf16 ? (double)to_f(static_cast<__nv_bfloat16 *>(h.db)[v]) : (double)static_cast<float *>(h.db)[v];
+	put(h.db, v, *h.error ? NAN : (float)s, h.bf16, 0);
 }
 
 /* ---- host --------------------------------------------------------------------------------------- */
@@ -281,6 +848,12 @@ int64_t up(int64_t n, int64_t to)
 
 /* where things lie in the workspace (byte offsets), and how the work is cut */
 struct head_plan {
+	size_t	x;		/* copies of x and w on a 16-byte grid, where needed */
+	size_t	w;
+	int	copy_x;
+	int	copy_w;
+	int64_t	ldx;
+	int64_t	ldw;
 	size_t	hit;
 	size_t	part;
 	size_t	row;
@@ -290,6 +863,8 @@ struct head_plan {
 	size_t	bytes;
 	int	piece;
 	int	terms;
+	int	splits;
+	int	ldd;
 };
 
 int check(const anni_head_call *c, int grad)
@@ -297,6 +872,8 @@ int check(const anni_head_call *c, int grad)
 	if (!c || c->tokens < 0 || c->d_model < 1 || c->vocab < 1)
 		return ANNI_E_ARG;
 	if (c->tokens > ANNI_HEAD_MAX_TOKENS || c->d_model > ANNI_HEAD_MAX_DIM || c->vocab > ANNI_HEAD_MAX_VOCAB)
+		return ANNI_E_LIMIT;
+	if ((up(c->tokens, HEAD_TM) / HEAD_TM) * (up(c->vocab, HEAD_TN) / HEAD_TN) > 0x3fffffff)
 		return ANNI_E_LIMIT;
 	if (c->ldx < c->d_model || c->ldw < c->vocab || ((uintptr_t)c->x & 1) || ((uintptr_t)c->w & 1))
 		return ANNI_E_ARG;
@@ -336,6 +913,12 @@ head_plan plan_of(const anni_head_call *c, int grad)
 
 	memset(&p, 0, sizeof(p));
 	p.bytes = 256;		/* the error word */
+	p.copy_x = grad || (c->ldx & 7) || ((uintptr_t)c->x & 15);
+	p.copy_w = (c->ldw & 7) || ((uintptr_t)c->w & 15);
+	p.ldx = up(c->d_model, 8);
+	p.ldw = up(c->vocab, 8);
+	p.x = take(&p.bytes, p.copy_x ? t * p.ldx * 2 : 0);
+	p.w = take(&p.bytes, p.copy_w ? c->d_model * p.ldw * 2 : 0);
 	if (!grad) {
 		p.hit = take(&p.bytes, t * 4);
 		p.part = take(&p.bytes, up(c->vocab, HEAD_TN) / HEAD_TN * t * 8);
@@ -346,8 +929,16 @@ head_plan plan_of(const anni_head_call *c, int grad)
 	    std::max<int64_t>(256, (int64_t)(HEAD_PIECE_BYTES / (size_t)(t * 2 * p.terms)) / 256 * 256));
 	p.row = take(&p.bytes, t * 4);
 	p.delta = take(&p.bytes, (int64_t)p.piece * t * 2 * p.terms);
-	p.dxp = take(&p.bytes, c->dx ? t * c->d_model * 4 : 0);
-	p.dbp = take(&p.bytes, up(t, HEAD_TM) / HEAD_TM * c->vocab * 4);
+	p.ldd = (int)up(c->d_model, 4);
+	p.splits = 1;
+	if (p.piece >= c->vocab) {
+		/* few tiles of dx and a long sum: cut the sum, at least four stages of it each */
+		const int64_t n = up(t, HEAD_TM) / HEAD_TM * (up(c->d_model, HEAD_TN) / HEAD_TN);
+
+		p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(HEAD_SMS / n, up(c->vocab, HEAD_TK) / HEAD_TK / 4));
+	}
+	p.dxp = take(&p.bytes, c->dx ? p.splits * t * p.ldd * 4 : 0);
+	p.dbp = take(&p.bytes, c->dbias ? up(t, HEAD_TM) / HEAD_TM * c->vocab * 4 : 0);
 	return p;
 }
 
@@ -357,10 +948,10 @@ head_args args_of(const anni_head_call *c, const head_plan &p)
 	char *ws = static_cast<char *>(c->workspace);
 
 	memset(&h, 0, sizeof(h));
-	h.x = static_cast<const __nv_bfloat16 *>(c->x);
-	h.ldx = c->ldx;
-	h.w = static_cast<const __nv_bfloat16 *>(c->w);
-	h.ldw = c->ldw;
+	h.x = p.copy_x ? reinterpret_cast<const __nv_bfloat16 *>(ws + p.x) : static_cast<const __nv_bfloat16 *>(c->x);
+	h.ldx = p.copy_x ? p.ldx : c->ldx;
+	h.w = p.copy_w ? reinterpret_cast<const __nv_bfloat16 *>(ws + p.w) : static_cast<const __nv_bfloat16 *>(c->w);
+	h.ldw = p.copy_w ? p.ldw : c->ldw;
 	h.bias = c->bias;
 	h.target = c->target;
 	h.weight = c->weight;
@@ -377,6 +968,8 @@ head_args args_of(const anni_head_call *c, const head_plan &p)
 	h.terms = p.terms;
 	h.ldp = p.piece;
 	h.dxp = reinterpret_cast<float *>(ws + p.dxp);
+	h.ldd = p.ldd;
+	h.splits = p.splits;
 	h.dbp = reinterpret_cast<float *>(ws + p.dbp);
 	h.dx = c->dx;
 	h.lddx = c->lddx;
@@ -398,6 +991,107 @@ int launched(void)
 {
 	anni_count_launch();
 	return cudaGetLastError() == cudaSuccess ? ANNI_OK : ANNI_E_CUDA;
+}
+
+typedef CUresult (*encode_fn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+    const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+    CUtensorMapFloatOOBfill);
+encode_fn g_encode;
+std::once_flag g_encode_once;
+
+void find_encode(void)
+{
+	void *p = NULL;
+	cudaDriverEntryPointQueryResult st;
+
+	if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &st) == cudaSuccess
+	    && st == cudaDriverEntryPointSuccess)
+		g_encode = reinterpret_cast<encode_fn>(p);
+	else
+		(void)cudaGetLastError();
+}
+
+/* bf16 [deep][rows][ld], of which `cols` columns exist, in boxes of 64 columns and `box` rows, 128-byte swizzle */
+int tensor_map(CUtensorMap *m, const void *base, int64_t cols, int64_t rows, int64_t ld, int deep, int box)
+{
+	const cuuint64_t dims[3] = { (cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)deep };
+	const cuuint64_t strides[2] = { (cuuint64_t)ld * 2, (cuuint64_t)ld * 2 * (cuuint64_t)rows };
+	const cuuint32_t boxes[3] = { 64, (cuuint32_t)box, 1 };
+	const cuuint32_t one[3] = { 1, 1, 1 };
+
+	std::call_once(g_encode_once, find_encode);
+	if (!g_encode)
+		return ANNI_E_CUDA;
+	return g_encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(base), dims, strides, boxes, one,
+	    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+	    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? ANNI_OK : ANNI_E_CUDA;
+}
+
+/* the product of one kind over the piece h.v0 .. h.v1 of the vocabulary */
+template <int KIND>
+int product(const head_args &h, cudaStream_t st)
+{
+	const int smem = HEAD_STAGES * HEAD_STAGE_BYTES + 1024;
+	const int width = h.v1 - h.v0;
+	gemm_args g;
+	int dev;
+	int sms;
+	int rc;
+
+	g.h = h;
+	if (KIND == LOSS || KIND == DELTA) {
+		g.m_tiles = (int)tiles(h.tokens, HEAD_TM);
+		g.n_tiles = (int)tiles(width, HEAD_TN);
+		g.k_blocks = (int)tiles(h.d, HEAD_TK);
+		rc = tensor_map(&g.a, h.x, h.d, h.tokens, h.ldx, 1, HEAD_TM);
+		rc = rc ? rc : tensor_map(&g.b, h.w, h.vocab, h.d, h.ldw, 1, HEAD_TK);
+	} else if (KIND == DX) {
+		g.m_tiles = (int)tiles(h.tokens, HEAD_TM);
+		g.n_tiles = (int)tiles(h.d, HEAD_TN);
+		g.k_blocks = (int)tiles(width, HEAD_TK);
+		rc = tensor_map(&g.a, h.delta, width, h.tokens, h.ldp, h.terms, HEAD_TM);
+		rc = rc ? rc : tensor_map(&g.b, h.w, h.vocab, h.d, h.ldw, 1, HEAD_TN);
+	} else {
+		g.m_tiles = (int)tiles(h.d, HEAD_TM);
+		g.n_tiles = (int)tiles(width, HEAD_TN);
+		g.k_blocks = (int)tiles(h.tokens, HEAD_TK);
+		rc = tensor_map(&g.a, h.x, h.d, h.tokens, h.ldx, 1, HEAD_TK);
+		rc = rc ? rc : tensor_map(&g.b, h.delta, width, h.tokens, h.ldp, h.terms, HEAD_TK);
+	}
+	if (rc != ANNI_OK)
+		return rc;
+	if (cudaGetDevice(&dev) != cudaSuccess
+	    || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess
+	    || cudaFuncSetAttribute(product_kernel<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+		(void)cudaGetLastError();
+		return ANNI_E_CUDA;
+	}
+	product_kernel<KIND><<<std::min(sms, g.m_tiles * g.n_tiles * (KIND == DX ? h.splits : 1)), HEAD_THREADS, smem, st>>>(g);
+	return launched();
+}
+
+/* the copies that the plan asks for; x's with the factors of the rows when gradients follow */
+int pack(const anni_head_call *c, const head_plan &p, const head_args &h, bool grad, cudaStream_t st)
+{
+	__nv_bfloat16 *x = const_cast<__nv_bfloat16 *>(h.x);
+	__nv_bfloat16 *w = const_cast<__nv_bfloat16 *>(h.w);
+	int rc = ANNI_OK;
+
+	if (grad || p.copy_x) {
+		const __nv_bfloat16 *from = static_cast<const __nv_bfloat16 *>(c->x);
+
+		if (grad)
+			pack_kernel<true><<<std::min(h.tokens, 8192), 128, 0, st>>>(h, x, h.ldx, from, c->ldx, h.tokens, h.d);
+		else
+			pack_kernel<false><<<std::min(h.tokens, 8192), 128, 0, st>>>(h, x, h.ldx, from, c->ldx, h.tokens, h.d);
+		rc = launched();
+	}
+	if (rc == ANNI_OK && p.copy_w) {
+		pack_kernel<false><<<std::min(h.d, 8192), 128, 0, st>>>(h, w, h.ldw, static_cast<const __nv_bfloat16 *>(c->w), c->ldw,
+		    h.d, h.vocab);
+		rc = launched();
+	}
+	return rc;
 }
 
 }	/* namespace */
@@ -428,10 +1122,12 @@ extern "C" int anni_head_loss(const anni_head_call *c, void *stream)
 	h = args_of(c, p);
 	if (cudaMemsetAsync(h.error, 0, 256, st) != cudaSuccess)
 		return ANNI_E_CUDA;
-	loss_kernel<<<dim3(tiles(h.vocab, HEAD_TN), tiles(h.tokens, HEAD_TM)), 256, 0, st>>>(h);
-	rc = launched();
+	rc = pack(c, p, h, false, st);
+	h.v1 = h.vocab;
+	if (rc == ANNI_OK)
+		rc = product<LOSS>(h, st);
 	if (rc == ANNI_OK) {
-		join_kernel<<<tiles(h.tokens, 256), 256, 0, st>>>(h, (int)tiles(h.vocab, HEAD_TN));
+		join_kernel<<<tiles(h.tokens, 32), 256, 0, st>>>(h, (int)tiles(h.vocab, HEAD_TN));
 		rc = launched();
 	}
 	return rc;
@@ -469,20 +1165,14 @@ extern "C" int anni_head_loss_grad(const anni_head_call *c, void *stream)
 	h = args_of(c, p);
 	if (cudaMemsetAsync(h.error, 0, 256, st) != cudaSuccess)
 		return ANNI_E_CUDA;
-	row_kernel<<<tiles(h.tokens, 256), 256, 0, st>>>(h);
-	rc = launched();
+	rc = pack(c, p, h, true, st);
 	for (h.v0 = 0; rc == ANNI_OK && h.v0 < h.vocab; h.v0 = h.v1) {
 		h.v1 = std::min(h.vocab, h.v0 + p.piece);
-		delta_kernel<<<dim3(tiles(h.v1 - h.v0, HEAD_TN), tiles(h.tokens, HEAD_TM)), 256, 0, st>>>(h);
-		rc = launched();
-		if (rc == ANNI_OK && h.dx) {
-			dx_kernel<<<dim3(tiles(h.d, HEAD_TN), tiles(h.tokens, HEAD_TM)), 256, 0, st>>>(h);
-			rc = launched();
-		}
-		if (rc == ANNI_OK && h.dw) {
-			dw_kernel<<<dim3(tiles(h.v1 - h.v0, HEAD_TN), tiles(h.d, HEAD_TM)), 256, 0, st>>>(h);
-			rc = launched();
-		}
+		rc = product<DELTA>(h, st);
+		if (rc == ANNI_OK && h.dx)
+			rc = product<DX>(h, st);
+		if (rc == ANNI_OK && h.dw)
+			rc = product<DW>(h, st);
 	}
 	if (rc == ANNI_OK && h.dx) {
 		finish_dx_kernel<<<std::min(2048u, tiles((int64_t)h.tokens * h.d, 256)), 256, 0, st>>>(h);

@@ -80,7 +80,8 @@ typedef struct anni_head_call {
 int	anni_head_workspace(const anni_head_call *c, int grad, size_t *bytes);
 /*
 ** nll and lse of every row.  ANNI_E_ARG: a missing or misaligned address, a size or stride out of range,
-** a workspace that is too small; nothing is queued then.
+** a workspace that is too small; ANNI_E_LIMIT: a size beyond its maximum, or more than 2^30 tiles of 128 rows
+** and 256 entries.  Nothing is queued then.
 */
 int	anni_head_loss(const anni_head_call *c, void *stream);
 /* dx, dw, dbias from lse, which an anni_head_loss on the same x, w, bias has written. */
