@@ -10,9 +10,11 @@
 **   dw      x^T delta of the piece, stored or added to the gradient
 ** Bound by the tensor cores: 2 T D V operations each (the logits twice, since they are not kept).
 **
-** A block (one per SM) works on 128 x 256 tiles: one thread loads tiles of both operands by TMA into a ring of
-** HEAD_STAGES stages, one thread issues tcgen05.mma into one of two accumulators in tensor memory, four warps
-** empty the other one.  An operand whose rows run along the summed dimension ("K-major") is loaded as one box
+** Two blocks (a cluster on two neighbouring SMs) work on a 256 x 256 tile: each keeps 128 rows of the result
+** and loads its 128 rows of the one operand and 128 of the other by TMA into a ring of HEAD_STAGES stages; one
+** thread of the first block issues tcgen05.mma for both SMs, which read half of the second operand from each
+** other's shared memory, into one of two accumulators in tensor memory, while four warps of each block empty
+** the other one.  An operand whose rows run along the summed dimension ("K-major") is loaded as one box
 ** of 64 k x rows, one whose rows run along the result ("MN-major") as boxes of 64 mn x 64 k, so nothing is
 ** transposed in memory.  Lengths that are no multiple of a tile end in zeros that TMA fills in.
 */
@@ -27,16 +29,17 @@
 #include "anni_head.h"
 #include "optstep_internal.h"
 
-#define HEAD_TM		128	/* rows and columns of a tile */
+#define HEAD_TM		256	/* rows and columns of a tile */
 #define HEAD_TN		256
+#define HEAD_HALF	128	/* rows of the result, and of either operand, in each block of the pair */
 #define HEAD_TK		64	/* 128 bytes of bf16: the widest swizzle */
-#define HEAD_STAGES	4
-#define HEAD_A_BYTES	(HEAD_TM * HEAD_TK * 2)
-#define HEAD_B_BYTES	(HEAD_TN * HEAD_TK * 2)
+#define HEAD_STAGES	6
+#define HEAD_A_BYTES	(HEAD_HALF * HEAD_TK * 2)
+#define HEAD_B_BYTES	(HEAD_HALF * HEAD_TK * 2)
 #define HEAD_STAGE_BYTES (HEAD_A_BYTES + HEAD_B_BYTES)
 #define HEAD_MN_BYTES	(64 * HEAD_TK * 2)	/* one MN-major box */
 #define HEAD_THREADS	256
-#define HEAD_SMS	148	/* what the work is cut for; any number of SMs runs it */
+#define HEAD_PAIRS	74	/* pairs of SMs that the work is cut for; any number of them runs it */
 #define HEAD_PIECE_BYTES ((size_t)192 << 20)	/* of delta in the workspace */
 #define HEAD_TERMS	3	/* bf16 terms of delta for fp32 gradients */
 #define HEAD_WAIT_NS	2000000000ull	/* a wait inside a kernel gives up after this long */
@@ -102,9 +105,18 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count)
 	asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(bar), "r"(count) : "memory");
 }
 
-__device__ __forceinline__ void mbar_arrive(uint32_t bar)
+/* the same variable in the shared memory of block `rank` of the cluster */
+__device__ __forceinline__ uint32_t smem_in(uint32_t addr, uint32_t rank)
 {
-	asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(bar) : "memory");
+	uint32_t r;
+
+	asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+	return r;
+}
+
+__device__ __forceinline__ void mbar_arrive_in(uint32_t cluster_bar)
+{
+	asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(cluster_bar) : "memory");
 }
 
 __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes)
@@ -116,7 +128,7 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity)
 {
 	uint32_t ok;
 
-	asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+	asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
 	    : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
 	return ok != 0;
 }
@@ -158,9 +170,10 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 	return mbar_try(bar, parity) || mbar_wait_long(bar, parity, stop, error);
 }
 
+/* into this block's memory, counted by a barrier of either block of the pair */
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1, int c2)
 {
-	asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+	asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
 	    :: "r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
 }
 
@@ -177,7 +190,7 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, bool mn)
 	return (uint64_t)((addr & 0x3ffff) >> 4) | lead << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
-/* D (fp32) = A B, both bf16: M 128, N 256, and which of them are MN-major */
+/* D (fp32) = A B, both bf16: M 256 and N 256 over the pair, and which of them are MN-major */
 __device__ __forceinline__ constexpr uint32_t instr_desc(bool a_mn, bool b_mn)
 {
 	return 1u << 4 | 1u << 7 | 1u << 10 | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | (uint32_t)(HEAD_TN >> 3) << 17
@@ -187,13 +200,15 @@ __device__ __forceinline__ constexpr uint32_t instr_desc(bool a_mn, bool b_mn)
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add)
 {
 	asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-	    "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+	    "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
 	    :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
 }
 
+/* arrives on this barrier of both blocks when the products issued so far are done */
 __device__ __forceinline__ void mma_commit(uint32_t bar)
 {
-	asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory");
+	asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+	    :: "r"(bar), "h"((uint16_t)3) : "memory");
 }
 
 /* 32 columns of this warp's 32 lanes of tensor memory: lane l gets row l */
@@ -230,6 +245,19 @@ __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi)
 	return *reinterpret_cast<const uint32_t *>(&q);
 }
 
+/* 32 bytes at a time: a whole sector per lane where each lane writes a row of its own */
+__device__ __forceinline__ void store32(void *p, const uint32_t (&r)[8])
+{
+	asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" :: "l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+	    "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
+
+__device__ __forceinline__ void load32(const void *p, uint32_t (&r)[8])
+{
+	asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]),
+	    "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "l"(p) : "memory");
+}
+
 __device__ __forceinline__ float to_f(__nv_bfloat16 v)
 {
 	return __bfloat162float(v);
@@ -240,20 +268,21 @@ __device__ __forceinline__ float to_f(__nv_bfloat16 v)
 /* ---- which tile, and what of it a stage holds ---------------------------------------------------- */
 
 struct tile_at {
-	int	m0;
+	int	m0;	/* this block's rows */
 	int	n0;
+	int	b0;	/* its share of the second operand */
 	int	k0;	/* k blocks lo .. hi - 1 of each term */
 	int	k1;
 	int	split;
 };
 
 /*
-** Order of the tiles.  loss, delta: all row tiles (64 at most) of one column tile after another, so that W is
+** Order of the tiles.  loss, delta: all row tiles (32 at most) of one column tile after another, so that W is
 ** read once while x stays in L2; dx: the column tiles of a row tile together, dw: the row tiles of a column tile
 ** together, so that delta is read once.
 */
 template <int KIND>
-__device__ __forceinline__ tile_at tile_of(const gemm_args &g, int t)
+__device__ __forceinline__ tile_at tile_of(const gemm_args &g, int t, int rank)
 {
 	tile_at r;
 	int m;
@@ -272,15 +301,16 @@ __device__ __forceinline__ tile_at tile_of(const gemm_args &g, int t)
 		m = t % g.m_tiles;
 		n = t / g.m_tiles;
 	} else {
-		const int group = t / (64 * g.n_tiles);
-		const int rows = min(64, g.m_tiles - group * 64);
-		const int i = t - group * 64 * g.n_tiles;
+		const int group = t / (32 * g.n_tiles);
+		const int rows = min(32, g.m_tiles - group * 32);
+		const int i = t - group * 32 * g.n_tiles;
 
-		m = group * 64 + i % rows;
+		m = group * 32 + i % rows;
 		n = i / rows;
 	}
-	r.m0 = m * HEAD_TM;
+	r.m0 = m * HEAD_TM + rank * HEAD_HALF;
 	r.n0 = n * HEAD_TN;
+	r.b0 = r.n0 + rank * HEAD_HALF;
 	return r;
 }
 
@@ -292,18 +322,18 @@ __device__ __forceinline__ void load_stage(const gemm_args &g, const tile_at &t,
 	if (KIND == LOSS || KIND == DELTA) {
 		tma_load(dst, &g.a, bar, k, t.m0, 0);
 #pragma unroll
-		for (int j = 0; j < HEAD_TN / 64; j++)
-			tma_load(b + j * HEAD_MN_BYTES, &g.b, bar, g.h.v0 + t.n0 + 64 * j, k, 0);
+		for (int j = 0; j < HEAD_HALF / 64; j++)
+			tma_load(b + j * HEAD_MN_BYTES, &g.b, bar, g.h.v0 + t.b0 + 64 * j, k, 0);
 	} else if (KIND == DX) {
 		tma_load(dst, &g.a, bar, k, t.m0, term);
-		tma_load(b, &g.b, bar, g.h.v0 + k, t.n0, 0);
+		tma_load(b, &g.b, bar, g.h.v0 + k, t.b0, 0);
 	} else {
 #pragma unroll
-		for (int j = 0; j < HEAD_TM / 64; j++)
+		for (int j = 0; j < HEAD_HALF / 64; j++)
 			tma_load(dst + j * HEAD_MN_BYTES, &g.a, bar, t.m0 + 64 * j, k, 0);
 #pragma unroll
-		for (int j = 0; j < HEAD_TN / 64; j++)
-			tma_load(b + j * HEAD_MN_BYTES, &g.b, bar, t.n0 + 64 * j, k, term);
+		for (int j = 0; j < HEAD_HALF / 64; j++)
+			tma_load(b + j * HEAD_MN_BYTES, &g.b, bar, t.b0 + 64 * j, k, term);
 	}
 }
 
@@ -438,17 +468,16 @@ __device__ __forceinline__ void delta_epilogue(const gemm_args &g, const tile_at
 				rest[i] = v[i];
 			/* the largest term last: the products add the small ones up first */
 			for (int k = h.terms - 1; k >= 0; k--) {
-				uint4 *q = reinterpret_cast<uint4 *>(out + (int64_t)k * h.tokens * h.ldp + c);
+				__nv_bfloat16 *q = out + (int64_t)k * h.tokens * h.ldp + c;
 
 #pragma unroll
-				for (int i = 0; i < 32; i += 8) {
-					uint4 r;
+				for (int i = 0; i < 32; i += 16) {
+					uint32_t r[8];
 
-					r.x = bf16_pair(rest[i], rest[i + 1]);
-					r.y = bf16_pair(rest[i + 2], rest[i + 3]);
-					r.z = bf16_pair(rest[i + 4], rest[i + 5]);
-					r.w = bf16_pair(rest[i + 6], rest[i + 7]);
-					q[i / 8] = r;
+#pragma unroll
+					for (int j = 0; j < 8; j++)
+						r[j] = bf16_pair(rest[i + 2 * j], rest[i + 2 * j + 1]);
+					store32(q + i, r);
 				}
 				if (k > 0)
 #pragma unroll
@@ -462,8 +491,8 @@ __device__ __forceinline__ void delta_epilogue(const gemm_args &g, const tile_at
 	if (h.db) {
 		epi_barrier();
 		for (int i = threadIdx.x & 127; i < HEAD_TN; i += 128)
-			if (h.v0 + at.n0 + i < h.v1)
-				h.dbp[(int64_t)(at.m0 / HEAD_TM) * h.vocab + h.v0 + at.n0 + i] =
+			if (at.m0 < h.tokens && h.v0 + at.n0 + i < h.v1)
+				h.dbp[(int64_t)(at.m0 / HEAD_HALF) * h.vocab + h.v0 + at.n0 + i] =
 				    (sums[0][i] + sums[1][i]) + (sums[2][i] + sums[3][i]);
 	}
 }
@@ -522,7 +551,7 @@ __device__ __forceinline__ void dw_epilogue(const gemm_args &g, const tile_at &a
 	const int size = h.bf16 ? 2 : 4;
 	const int64_t first = (int64_t)d * h.lddw + v0;
 	char *out = static_cast<char *>(h.dw) + first * size;
-	const bool vec = ((uintptr_t)out & 15) == 0;
+	const bool vec = ((uintptr_t)out & 31) == 0;
 
 #pragma unroll 1
 	for (int c = 0; c < HEAD_TN && v0 + c < h.v1; c += 32) {
@@ -537,34 +566,31 @@ __device__ __forceinline__ void dw_epilogue(const gemm_args &g, const tile_at &a
 				if (v0 + c + i < h.v1)
 					put(h.dw, first + c + i, v[i], h.bf16, h.add);
 		} else if (h.bf16) {
-			uint4 *q = reinterpret_cast<uint4 *>(out + c * 2);
-
 #pragma unroll
-			for (int i = 0; i < 32; i += 8) {
-				uint4 r = h.add ? q[i / 8] : make_uint4(0, 0, 0, 0);
-				const float2 r0 = unpack2(r.x);
-				const float2 r1 = unpack2(r.y);
-				const float2 r2 = unpack2(r.z);
-				const float2 r3 = unpack2(r.w);
+			for (int i = 0; i < 32; i += 16) {
+				uint32_t r[8] = { 0, 0, 0, 0, 0, 0, 0, 0 };
 
-				r.x = bf16_pair(r0.x + v[i], r0.y + v[i + 1]);
-				r.y = bf16_pair(r1.x + v[i + 2], r1.y + v[i + 3]);
-				r.z = bf16_pair(r2.x + v[i + 4], r2.y + v[i + 5]);
-				r.w = bf16_pair(r3.x + v[i + 6], r3.y + v[i + 7]);
-				q[i / 8] = r;
+				if (h.add)
+					load32(out + (c + i) * 2, r);
+#pragma unroll
+				for (int j = 0; j < 8; j++) {
+					const float2 q = unpack2(r[j]);
+
+					r[j] = bf16_pair(q.x + v[i + 2 * j], q.y + v[i + 2 * j + 1]);
+				}
+				store32(out + (c + i) * 2, r);
 			}
 		} else {
-			float4 *q = reinterpret_cast<float4 *>(out + c * 4);
-
 #pragma unroll
-			for (int i = 0; i < 32; i += 4) {
-				float4 r = h.add ? q[i / 4] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+			for (int i = 0; i < 32; i += 8) {
+				uint32_t r[8] = { 0, 0, 0, 0, 0, 0, 0, 0 };
 
-				r.x += v[i];
-				r.y += v[i + 1];
-				r.z += v[i + 2];
-				r.w += v[i + 3];
-				q[i / 4] = r;
+				if (h.add)
+					load32(out + (c + i) * 4, r);
+#pragma unroll
+				for (int j = 0; j < 8; j++)
+					r[j] = __float_as_uint(__uint_as_float(r[j]) + v[i + j]);
+				store32(out + (c + i) * 4, r);
 			}
 		}
 	}
@@ -583,34 +609,45 @@ struct gemm_smem {
 	epi_smem	epi;
 };
 
-/* loads; returns after a give-up only when its own copies have landed (or the time is up) */
+/*
+** Loads this block's shares.  The first block's barrier counts both blocks' bytes, since the products of both
+** are issued there.  Returns after a give-up only when the copies in flight have landed, or the time is up.
+*/
 template <int KIND>
-__device__ __forceinline__ void producer(const gemm_args &g, gemm_smem *s, uint32_t ring, int total)
+__device__ __forceinline__ void producer(const gemm_args &g, gemm_smem *s, uint32_t ring, int total, int rank, int pair, int pairs)
 {
 	uint32_t n = 0;		/* stages loaded so far */
 
-	for (int tile = blockIdx.x; tile < total; tile += gridDim.x) {
-		const tile_at at = tile_of<KIND>(g, tile);
+	for (int tile = pair; tile < total; tile += pairs) {
+		const tile_at at = tile_of<KIND>(g, tile, rank);
 
 		for (int term = 0; term < (KIND == DX || KIND == DW ? g.h.terms : 1); term++)
 			for (int k = at.k0; k < at.k1; k++, n++) {
 				const uint32_t i = n % HEAD_STAGES;
 
 				if (!mbar_wait(smem_of(&s->empty[i]), (n / HEAD_STAGES & 1) ^ 1, &s->stop, g.h.error)) {
-					for (uint32_t j = n < HEAD_STAGES ? 0 : n - HEAD_STAGES; j < n; j++)
-						(void)mbar_wait(smem_of(&s->full[j % HEAD_STAGES]), j / HEAD_STAGES & 1, NULL,
-						    g.h.error);
+					if (rank == 0)
+						for (uint32_t j = n < HEAD_STAGES ? 0 : n - HEAD_STAGES; j < n; j++)
+							(void)mbar_wait(smem_of(&s->full[j % HEAD_STAGES]),
+							    j / HEAD_STAGES & 1, NULL, g.h.error);
+					else {
+						/* counted elsewhere: no copy is under way for this long */
+						for (const uint64_t end = now_ns() + HEAD_WAIT_NS / 100; now_ns() < end; )
+							__nanosleep(1000);
+					}
 					return;
 				}
-				mbar_expect(smem_of(&s->full[i]), HEAD_STAGE_BYTES);
+				if (rank == 0)
+					mbar_expect(smem_of(&s->full[i]), 2 * HEAD_STAGE_BYTES);
 				load_stage<KIND>(g, at, KIND == DX || KIND == DW ? g.h.terms - 1 - term : 0, k * HEAD_TK,
-				    ring + i * HEAD_STAGE_BYTES, smem_of(&s->full[i]));
+				    ring + i * HEAD_STAGE_BYTES, smem_in(smem_of(&s->full[i]), 0));
 			}
 	}
 }
 
+/* the first block's: issues the products of both */
 template <int KIND>
-__device__ __forceinline__ void multiplier(const gemm_args &g, gemm_smem *s, uint32_t ring, int total)
+__device__ __forceinline__ void multiplier(const gemm_args &g, gemm_smem *s, uint32_t ring, int total, int pair, int pairs)
 {
 	const bool a_mn = KIND == DW;
 	const bool b_mn = KIND != DX;
@@ -618,8 +655,8 @@ __device__ __forceinline__ void multiplier(const gemm_args &g, gemm_smem *s, uin
 	uint32_t n = 0;
 	uint32_t done = 0;	/* tiles */
 
-	for (int tile = blockIdx.x; tile < total; tile += gridDim.x, done++) {
-		const tile_at at = tile_of<KIND>(g, tile);
+	for (int tile = pair; tile < total; tile += pairs, done++) {
+		const tile_at at = tile_of<KIND>(g, tile, 0);
 		const int steps = (at.k1 - at.k0) * (KIND == DX || KIND == DW ? g.h.terms : 1);
 		const uint32_t acc = s->tmem + (done & 1) * HEAD_TN;
 		bool ok = mbar_wait(smem_of(&s->drained[done & 1]), (done / 2 & 1) ^ 1, &s->stop, g.h.error);
@@ -650,13 +687,13 @@ __device__ __forceinline__ void multiplier(const gemm_args &g, gemm_smem *s, uin
 }
 
 template <int KIND>
-__device__ __forceinline__ void drainer(const gemm_args &g, gemm_smem *s, int total)
+__device__ __forceinline__ void drainer(const gemm_args &g, gemm_smem *s, int total, int rank, int pair, int pairs)
 {
 	const uint32_t lanes = (uint32_t)(threadIdx.x >> 5 & 3) << 21;	/* this warp's quarter of the lanes: 32 w << 16 */
 	uint32_t done = 0;
 
-	for (int tile = blockIdx.x; tile < total; tile += gridDim.x, done++) {
-		const tile_at at = tile_of<KIND>(g, tile);
+	for (int tile = pair; tile < total; tile += pairs, done++) {
+		const tile_at at = tile_of<KIND>(g, tile, rank);
 		const uint32_t b = done & 1;
 		const uint32_t acc = s->tmem + lanes + b * HEAD_TN;
 
@@ -679,17 +716,25 @@ __device__ __forceinline__ void drainer(const gemm_args &g, gemm_smem *s, int to
 		asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 		__syncwarp();
 		if ((threadIdx.x & 31) == 0)
-			mbar_arrive(smem_of(&s->drained[b]));
+			mbar_arrive_in(smem_in(smem_of(&s->drained[b]), 0));
 	}
 }
 
+__device__ __forceinline__ void cluster_barrier(void)
+{
+	asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 template <int KIND>
-__global__ void __launch_bounds__(HEAD_THREADS, 1) product_kernel(const __grid_constant__ gemm_args g)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HEAD_THREADS, 1) product_kernel(const __grid_constant__ gemm_args g)
 {
 	extern __shared__ uint8_t dynamic[];
 	__shared__ gemm_smem s;
 	const uint32_t ring = (smem_of(dynamic) + 1023) & ~1023u;	/* swizzle atoms lie on 1024 bytes */
 	const int warp = threadIdx.x >> 5;
+	const int rank = blockIdx.x & 1;
+	const int pair = blockIdx.x >> 1;
+	const int pairs = gridDim.x >> 1;
 	const int total = g.m_tiles * g.n_tiles * (KIND == DX ? g.h.splits : 1);
 
 	if (threadIdx.x == 0) {
@@ -699,75 +744,81 @@ __global__ void __launch_bounds__(HEAD_THREADS, 1) product_kernel(const __grid_c
 		}
 		for (int i = 0; i < 2; i++) {
 			mbar_init(smem_of(&s.ready[i]), 1);
-			mbar_init(smem_of(&s.drained[i]), 4);
+			mbar_init(smem_of(&s.drained[i]), 8);	/* four warps of either block */
 		}
 		mbar_init(smem_of(&s.quiet), 1);
 		s.stop = 0;
 		asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 		asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 	}
+	__syncwarp();
 	if (warp == 2) {
-		asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" :: "r"(smem_of(&s.tmem)) : "memory");
-		asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+		asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" :: "r"(smem_of(&s.tmem)) : "memory");
+		asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
 	}
 	asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 	__syncthreads();
+	cluster_barrier();
 	asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 	if (warp == 0) {
 		if ((threadIdx.x & 31) == 0)
-			producer<KIND>(g, &s, ring, total);
-		__syncwarp();
+			producer<KIND>(g, &s, ring, total, rank, pair, pairs);
 	} else if (warp == 1) {
-		if ((threadIdx.x & 31) == 0)
-			multiplier<KIND>(g, &s, ring, total);
-		__syncwarp();
+		if ((threadIdx.x & 31) == 0 && rank == 0)
+			multiplier<KIND>(g, &s, ring, total, pair, pairs);
 	} else if (warp >= 4)
-		drainer<KIND>(g, &s, total);
+		drainer<KIND>(g, &s, total, rank, pair, pairs);
+	__syncwarp();
 	asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 	__syncthreads();
+	cluster_barrier();	/* neither block leaves, nor gives its tensor memory back, while the other may need it */
 	asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 	if (warp == 2)
-		asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" :: "r"(s.tmem) : "memory");
+		asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" :: "r"(s.tmem) : "memory");
 }
 
 /* ---- what goes before and after the products ------------------------------------------------------------ */
 
-/* joins the tiles of a row: eight warps share the tiles of 32 rows */
-__global__ void __launch_bounds__(256) join_kernel(const head_args h, int tiles)
+/* joins the tiles of a row: 32 warps share the tiles of 32 rows */
+__device__ __forceinline__ void join(float &top, float &sum, float2 p)
 {
-	__shared__ float2 s[8][32];
-	const int t = blockIdx.x * 32 + (threadIdx.x & 31);
+	const float high = fmaxf(top, p.x);
+	const float base = high == -INFINITY ? 0.0f : high;
+
+	sum = sum * exp2f((top - base) * LOG2E) + p.y * exp2f((p.x - base) * LOG2E);
+	top = high;
+}
+
+__global__ void __launch_bounds__(1024) join_kernel(const head_args h, int tiles)
+{
+	__shared__ float2 s[32][33];
+	const int lane = threadIdx.x & 31;
 	const int w = threadIdx.x >> 5;
+	int t = blockIdx.x * 32 + lane;
 	float top = -INFINITY;
 	float sum = 0.0f;
-	float lse;
-	int y;
 
-	if (t < h.tokens)
-		for (int k = w; k < tiles; k += 8) {
-			const float2 p = h.part[(int64_t)k * h.tokens + t];
-			const float high = fmaxf(top, p.x);
-			const float base = high == -INFINITY ? 0.0f : high;
-
-			sum = sum * exp2f((top - base) * LOG2E) + p.y * exp2f((p.x - base) * LOG2E);
-			top = high;
-		}
-	s[w][threadIdx.x & 31] = make_float2(top, sum);
-	__syncthreads();
-	if (w != 0 || t >= h.tokens)
-		return;
-	for (int k = 1; k < 8; k++) {
-		const float2 p = s[k][threadIdx.x];
-		const float high = fmaxf(top, p.x);
-		const float base = high == -INFINITY ? 0.0f : high;
-
-		sum = sum * exp2f((top - base) * LOG2E) + p.y * exp2f((p.x - base) * LOG2E);
-		top = high;
+	if (t < h.tokens) {
+#pragma unroll 4
+		for (int k = w; k < tiles; k += 32)
+			join(top, sum, h.part[(int64_t)k * h.tokens + t]);
 	}
-	lse = *h.error ? NAN : top + logf(sum);
-	y = h.target[t];
-	h.lse[t] = lse;
-	h.nll[t] = y < 0 ? (*h.error ? NAN : 0.0f) : y >= h.vocab ? NAN : lse - h.hit[t];
+	s[lane][w] = make_float2(top, sum);
+	__syncthreads();
+	/* warp w now joins row w */
+	t = blockIdx.x * 32 + w;
+	top = s[w][lane].x;
+	sum = s[w][lane].y;
+#pragma unroll
+	for (int k = 16; k > 0; k >>= 1)
+		join(top, sum, make_float2(__shfl_down_sync(0xffffffffu, top, k), __shfl_down_sync(0xffffffffu, sum, k)));
+	if (lane == 0 && t < h.tokens) {
+		const float lse = *h.error ? NAN : top + logf(sum);
+		const int y = h.target[t];
+
+		h.lse[t] = lse;
+		h.nll[t] = y < 0 ? (*h.error ? NAN : 0.0f) : y >= h.vocab ? NAN : lse - h.hit[t];
+	}
 }
 
 /* factor of each row: 0 where there is no gradient */
@@ -809,19 +860,42 @@ __global__ void __launch_bounds__(128) pack_kernel(const head_args h, __nv_bfloa
 	}
 }
 
-__global__ void __launch_bounds__(256) finish_dx_kernel(const head_args h)
+/* the parts of dx added up in order; a block takes a row at a time */
+__global__ void __launch_bounds__(128) finish_dx_kernel(const head_args h)
 {
 	const bool bad = *h.error != 0;
 
-	for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < (int64_t)h.tokens * h.d;
-	    i += (int64_t)gridDim.x * blockDim.x) {
-		const int64_t t = i / h.d;
-		const int64_t d = i - t * h.d;
-		float v = 0.0f;
+	for (int t = blockIdx.x; t < h.tokens; t += gridDim.x) {
+		const int size = h.bf16 ? 2 : 4;
+		char *out = static_cast<char *>(h.dx) + (int64_t)t * h.lddx * size;
 
-		for (int k = 0; k < h.splits; k++)
-			v += h.dxp[((int64_t)k * h.tokens + t) * h.ldd + d];
-		put(h.dx, t * h.lddx + d, bad ? NAN : v, h.bf16, 0);
+		for (int d = threadIdx.x * 4; d < h.d; d += 128 * 4) {
+			float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+
+			for (int k = 0; k < h.splits; k++) {
+				const float4 q = *reinterpret_cast<const float4 *>(h.dxp + ((int64_t)k * h.tokens + t) * h.ldd + d);
+
+				v.x += q.x;
+				v.y += q.y;
+				v.z += q.z;
+				v.w += q.w;
+			}
+			if (bad)
+				v = make_float4(NAN, NAN, NAN, NAN);
+			if (d + 4 <= h.d && ((uintptr_t)out & 15) == 0) {
+				if (h.bf16)
+					*reinterpret_cast<uint2 *>(out + d * 2) = make_uint2(bf16_pair(v.x, v.y), bf16_pair(v.z, v.w));
+				else
+					*reinterpret_cast<float4 *>(out + d * 4) = v;
+			} else {
+				const float e[4] = { v.x, v.y, v.z, v.w };
+
+#pragma unroll
+				for (int j = 0; j < 4; j++)
+					if (d + j < h.d)
+						put(out, d + j, e[j], h.bf16, 0);
+			}
+		}
 	}
 }
 
@@ -906,6 +980,30 @@ size_t take(size_t *at, int64_t bytes)
 	return here;
 }
 
+/*
+** Into how many parts the sum over the vocabulary in dx is cut: the number of tiles of dx does not depend on the
+** vocabulary, and often leaves pairs of SMs idle in the last round.  The fewest parts, of at least eight stages,
+** whose rounds waste the least.  (4096 rows of 1536: 96 tiles are two rounds of 74 pairs, 65 % used; three parts
+** make four shorter rounds, 97 %.)
+*/
+int split_dx(int64_t tiles_of_dx, int64_t stages)
+{
+	int best = 1;
+	double least = 1e30;
+
+	for (int s = 1; s <= HEAD_PAIRS && (s == 1 || stages / s >= 8); s++) {
+		const double rounds = (double)up(tiles_of_dx * s, HEAD_PAIRS) / HEAD_PAIRS / s;
+
+		if (s > 4 && tiles_of_dx >= HEAD_PAIRS)
+			break;		/* each part costs a pass over an fp32 copy of dx */
+		if (rounds < least * 0.97) {
+			least = rounds;
+			best = s;
+		}
+	}
+	return best;
+}
+
 head_plan plan_of(const anni_head_call *c, int grad)
 {
 	head_plan p;
@@ -930,15 +1028,10 @@ head_plan plan_of(const anni_head_call *c, int grad)
 	p.row = take(&p.bytes, t * 4);
 	p.delta = take(&p.bytes, (int64_t)p.piece * t * 2 * p.terms);
 	p.ldd = (int)up(c->d_model, 4);
-	p.splits = 1;
-	if (p.piece >= c->vocab) {
-		/* few tiles of dx and a long sum: cut the sum, at least four stages of it each */
-		const int64_t n = up(t, HEAD_TM) / HEAD_TM * (up(c->d_model, HEAD_TN) / HEAD_TN);
-
-		p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(HEAD_SMS / n, up(c->vocab, HEAD_TK) / HEAD_TK / 4));
-	}
+	p.splits = split_dx(up(t, HEAD_TM) / HEAD_TM * (up(c->d_model, HEAD_TN) / HEAD_TN),
+	    up(std::min(p.piece, c->vocab), HEAD_TK) / HEAD_TK);
 	p.dxp = take(&p.bytes, c->dx ? p.splits * t * p.ldd * 4 : 0);
-	p.dbp = take(&p.bytes, c->dbias ? up(t, HEAD_TM) / HEAD_TM * c->vocab * 4 : 0);
+	p.dbp = take(&p.bytes, c->dbias ? up(t, HEAD_HALF) / HEAD_HALF * c->vocab * 4 : 0);
 	return p;
 }
 
@@ -1043,14 +1136,14 @@ int product(const head_args &h, cudaStream_t st)
 		g.m_tiles = (int)tiles(h.tokens, HEAD_TM);
 		g.n_tiles = (int)tiles(width, HEAD_TN);
 		g.k_blocks = (int)tiles(h.d, HEAD_TK);
-		rc = tensor_map(&g.a, h.x, h.d, h.tokens, h.ldx, 1, HEAD_TM);
+		rc = tensor_map(&g.a, h.x, h.d, h.tokens, h.ldx, 1, HEAD_HALF);
 		rc = rc ? rc : tensor_map(&g.b, h.w, h.vocab, h.d, h.ldw, 1, HEAD_TK);
 	} else if (KIND == DX) {
 		g.m_tiles = (int)tiles(h.tokens, HEAD_TM);
 		g.n_tiles = (int)tiles(h.d, HEAD_TN);
 		g.k_blocks = (int)tiles(width, HEAD_TK);
-		rc = tensor_map(&g.a, h.delta, width, h.tokens, h.ldp, h.terms, HEAD_TM);
-		rc = rc ? rc : tensor_map(&g.b, h.w, h.vocab, h.d, h.ldw, 1, HEAD_TN);
+		rc = tensor_map(&g.a, h.delta, width, h.tokens, h.ldp, h.terms, HEAD_HALF);
+		rc = rc ? rc : tensor_map(&g.b, h.w, h.vocab, h.d, h.ldw, 1, HEAD_HALF);
 	} else {
 		g.m_tiles = (int)tiles(h.d, HEAD_TM);
 		g.n_tiles = (int)tiles(width, HEAD_TN);
@@ -1066,7 +1159,7 @@ int product(const head_args &h, cudaStream_t st)
 		(void)cudaGetLastError();
 		return ANNI_E_CUDA;
 	}
-	product_kernel<KIND><<<std::min(sms, g.m_tiles * g.n_tiles * (KIND == DX ? h.splits : 1)), HEAD_THREADS, smem, st>>>(g);
+	product_kernel<KIND><<<2 * std::min(sms / 2, g.m_tiles * g.n_tiles * (KIND == DX ? h.splits : 1)), HEAD_THREADS, smem, st>>>(g);
 	return launched();
 }
 
@@ -1127,7 +1220,7 @@ extern "C" int anni_head_loss(const anni_head_call *c, void *stream)
 	if (rc == ANNI_OK)
 		rc = product<LOSS>(h, st);
 	if (rc == ANNI_OK) {
-		join_kernel<<<tiles(h.tokens, 32), 256, 0, st>>>(h, (int)tiles(h.vocab, HEAD_TN));
+		join_kernel<<<tiles(h.tokens, 32), 1024, 0, st>>>(h, (int)tiles(h.vocab, HEAD_TN));
 		rc = launched();
 	}
 	return rc;
@@ -1175,11 +1268,11 @@ extern "C" int anni_head_loss_grad(const anni_head_call *c, void *stream)
 			rc = product<DW>(h, st);
 	}
 	if (rc == ANNI_OK && h.dx) {
-		finish_dx_kernel<<<std::min(2048u, tiles((int64_t)h.tokens * h.d, 256)), 256, 0, st>>>(h);
+		finish_dx_kernel<<<std::min(h.tokens, 16384), 128, 0, st>>>(h);
 		rc = launched();
 	}
 	if (rc == ANNI_OK && h.db) {
-		finish_db_kernel<<<tiles(h.vocab, 256), 256, 0, st>>>(h, (int)tiles(h.tokens, HEAD_TM));
+		finish_db_kernel<<<tiles(h.vocab, 256), 256, 0, st>>>(h, (int)tiles(h.tokens, HEAD_HALF));
 		rc = launched();
 	}
 	return rc;
