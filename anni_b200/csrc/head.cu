@@ -25,6 +25,7 @@
 #include <stdint.h>
 #include <string.h>
 #include <algorithm>
+#include <atomic>
 #include <mutex>
 #include "anni_head.h"
 #include "optstep_internal.h"
@@ -40,7 +41,7 @@
 #define HEAD_MN_BYTES	(64 * HEAD_TK * 2)	/* one MN-major box */
 #define HEAD_THREADS	256
 #define HEAD_PAIRS	74	/* pairs of SMs that the work is cut for; any number of them runs it */
-#define HEAD_PIECE_BYTES ((size_t)192 << 20)	/* of delta in the workspace */
+#define HEAD_PIECE_BYTES ((size_t)256 << 20)	/* of delta in the workspace */
 #define HEAD_TERMS	3	/* bf16 terms of delta for fp32 gradients */
 #define HEAD_WAIT_NS	2000000000ull	/* a wait inside a kernel gives up after this long */
 
@@ -70,7 +71,7 @@ struct head_args {
 	int64_t			ldp;
 	int			v0;		/* the piece: columns v0 .. v1 - 1 */
 	int			v1;
-	float			*dxp;		/* fp32 [splits][tokens][ldd] */
+	float			*dxp;		/* fp32 [splits][tokens][ldd], or NULL: straight into dx */
 	int			ldd;
 	int			splits;
 	float			*dbp;		/* fp32 [row tiles][vocab] */
@@ -81,7 +82,6 @@ struct head_args {
 	void			*db;
 	int			bf16;
 	int			add;
-	int			*error;
 };
 
 struct gemm_args {
@@ -142,11 +142,11 @@ __device__ __forceinline__ uint64_t now_ns(void)
 }
 
 /*
-** Waits for the barrier's phase of this parity.  Gives up, and says so to the whole block through `stop` and to
-** the host through `error`, after HEAD_WAIT_NS, or as soon as another thread of the block has given up
-** (stop NULL: only the time counts).
+** Waits for the barrier's phase of this parity.  Gives up, and says so to the whole block through `stop`, after
+** HEAD_WAIT_NS, or as soon as another thread of the block has given up (stop NULL: only the time counts).  What a
+** block has not computed by then it fills with NaN.
 */
-__device__ __noinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity, volatile int *stop, int *error)
+__device__ __noinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity, volatile int *stop)
 {
 	const uint64_t end = now_ns() + HEAD_WAIT_NS;
 
@@ -159,15 +159,14 @@ __device__ __noinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity, volat
 		if (now_ns() > end) {
 			if (stop)
 				*stop = 1;
-			atomicExch(error, ANNI_E_BARRIER_TIMEOUT);
 			return false;
 		}
 	}
 }
 
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *stop, int *error)
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *stop)
 {
-	return mbar_try(bar, parity) || mbar_wait_long(bar, parity, stop, error);
+	return mbar_try(bar, parity) || mbar_wait_long(bar, parity, stop);
 }
 
 /* into this block's memory, counted by a barrier of either block of the pair */
@@ -211,8 +210,8 @@ __device__ __forceinline__ void mma_commit(uint32_t bar)
 	    :: "r"(bar), "h"((uint16_t)3) : "memory");
 }
 
-/* 32 columns of this warp's 32 lanes of tensor memory: lane l gets row l */
-__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32])
+/* 32 columns of this warp's 32 lanes of tensor memory: lane l gets row l (ok false: NaN) */
+__device__ __forceinline__ void tmem_load(uint32_t addr, bool ok, float (&v)[32])
 {
 	uint32_t r[32];
 
@@ -227,7 +226,7 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32])
 	asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
 	for (int i = 0; i < 32; i++)
-		v[i] = __uint_as_float(r[i]);
+		v[i] = ok ? __uint_as_float(r[i]) : NAN;
 }
 
 __device__ __forceinline__ float exp2_approx(float x)
@@ -378,7 +377,7 @@ __device__ __forceinline__ float column_sums(float (&v)[32])
 }
 
 /* one pass over the columns with a running maximum and a sum that follows it */
-__device__ __forceinline__ void loss_epilogue(const gemm_args &g, const tile_at &at, uint32_t tmem, const float *bias)
+__device__ __forceinline__ void loss_epilogue(const gemm_args &g, const tile_at &at, uint32_t tmem, bool ok, const float *bias)
 {
 	const head_args &h = g.h;
 	const int t = at.m0 + (threadIdx.x & 127);
@@ -393,7 +392,7 @@ __device__ __forceinline__ void loss_epilogue(const gemm_args &g, const tile_at 
 		float high;
 		float base;
 
-		tmem_load(tmem + c, v);
+		tmem_load(tmem + c, ok, v);
 #pragma unroll
 		for (int i = 0; i < 32; i += 4) {
 			const float4 b = *reinterpret_cast<const float4 *>(bias + c + i);
@@ -412,7 +411,7 @@ __device__ __forceinline__ void loss_epilogue(const gemm_args &g, const tile_at 
 		high = v[0];
 #pragma unroll
 		for (int i = 1; i < 32; i++)
-			high = fmaxf(high, v[i]);
+			high = fmaxf(high, v[i]);	/* a NaN shows in the sum */
 		high = fmaxf(high, top);
 		base = high == -INFINITY ? 0.0f : high;
 		sum *= exp2_approx((top - base) * LOG2E);
@@ -425,7 +424,7 @@ __device__ __forceinline__ void loss_epilogue(const gemm_args &g, const tile_at 
 		h.part[(int64_t)(at.n0 / HEAD_TN) * h.tokens + t] = make_float2(top, sum);
 }
 
-__device__ __forceinline__ void delta_epilogue(const gemm_args &g, const tile_at &at, uint32_t tmem, const float *bias,
+__device__ __forceinline__ void delta_epilogue(const gemm_args &g, const tile_at &at, uint32_t tmem, bool ok, const float *bias,
 	float (*sums)[HEAD_TN])
 {
 	const head_args &h = g.h;
@@ -441,7 +440,7 @@ __device__ __forceinline__ void delta_epilogue(const gemm_args &g, const tile_at
 	for (int c = 0; c < HEAD_TN; c += 32) {
 		float v[32];
 
-		tmem_load(tmem + c, v);
+		tmem_load(tmem + c, ok, v);
 #pragma unroll
 		for (int i = 0; i < 32; i += 4) {
 			const float4 b = *reinterpret_cast<const float4 *>(bias + c + i);
@@ -497,34 +496,6 @@ __device__ __forceinline__ void delta_epilogue(const gemm_args &g, const tile_at
 	}
 }
 
-__device__ __forceinline__ void dx_epilogue(const gemm_args &g, const tile_at &at, uint32_t tmem)
-{
-	const head_args &h = g.h;
-	const int t = at.m0 + (threadIdx.x & 127);
-	float *out = h.dxp + ((int64_t)at.split * h.tokens + t) * h.ldd + at.n0;
-
-#pragma unroll 1
-	for (int c = 0; c < HEAD_TN && at.n0 + c < h.ldd; c += 32) {
-		float v[32];
-
-		tmem_load(tmem + c, v);
-		if (t >= h.tokens)
-			continue;
-#pragma unroll
-		for (int i = 0; i < 32; i += 4)
-			if (at.n0 + c + i < h.ldd) {
-				float4 *q = reinterpret_cast<float4 *>(out + c + i);
-				float4 r = h.v0 ? *q : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-
-				r.x += v[i];
-				r.y += v[i + 1];
-				r.z += v[i + 2];
-				r.w += v[i + 3];
-				*q = r;
-			}
-	}
-}
-
 __device__ __forceinline__ void put(void *base, int64_t i, float v, int bf16, int add)
 {
 	if (bf16) {
@@ -543,56 +514,81 @@ __device__ __forceinline__ float2 unpack2(uint32_t q)
 	return make_float2(__uint_as_float(q << 16), __uint_as_float(q & 0xffff0000u));
 }
 
-__device__ __forceinline__ void dw_epilogue(const gemm_args &g, const tile_at &at, uint32_t tmem)
+/*
+** Eight or sixteen consecutive results (32 bytes) of a row, stored or added to what is there, element by element where
+** the row ends or its address is not on 32 bytes.
+*/
+template <typename T, int N>
+__device__ __forceinline__ void put_some(T *out, const float *v, int left, bool add)
+{
+	if (left >= N && ((uintptr_t)out & 31) == 0) {
+		uint32_t r[8] = { 0, 0, 0, 0, 0, 0, 0, 0 };
+
+		if (add)
+			load32(out, r);
+#pragma unroll
+		for (int j = 0; j < 8; j++)
+			if (N == 16) {
+				const float2 q = unpack2(r[j]);
+
+				r[j] = bf16_pair(q.x + v[2 * j % N], q.y + v[(2 * j + 1) % N]);
+			} else
+				r[j] = __float_as_uint(__uint_as_float(r[j]) + v[j]);
+		store32(out, r);
+		return;
+	}
+#pragma unroll
+	for (int j = 0; j < N; j++)
+		if (j < left)
+			put(out, j, v[j], N == 16, add);
+}
+
+/* 32 columns of a row of a matrix of the gradients' type, `left` of which exist */
+__device__ __forceinline__ void put_row(void *base, int64_t first, const float (&v)[32], int left, bool bf16, bool add)
+{
+	if (bf16) {
+#pragma unroll
+		for (int i = 0; i < 32; i += 16)
+			put_some<__nv_bfloat16, 16>(static_cast<__nv_bfloat16 *>(base) + first + i, v + i, left - i, add);
+	} else {
+#pragma unroll
+		for (int i = 0; i < 32; i += 8)
+			put_some<float, 8>(static_cast<float *>(base) + first + i, v + i, left - i, add);
+	}
+}
+
+__device__ __forceinline__ void dx_epilogue(const gemm_args &g, const tile_at &at, uint32_t tmem, bool ok)
+{
+	const head_args &h = g.h;
+	const int t = at.m0 + (threadIdx.x & 127);
+
+#pragma unroll 1
+	for (int c = 0; c < HEAD_TN && at.n0 + c < h.d; c += 32) {
+		float v[32];
+
+		tmem_load(tmem + c, ok, v);
+		if (t >= h.tokens)
+			continue;
+		if (h.dxp)
+			put_row(h.dxp, ((int64_t)at.split * h.tokens + t) * h.ldd + at.n0 + c, v, h.ldd - at.n0 - c, false, h.v0 != 0);
+		else		/* one part, one piece: that is dx */
+			put_row(h.dx, t * h.lddx + at.n0 + c, v, h.d - at.n0 - c, h.bf16, false);
+	}
+}
+
+__device__ __forceinline__ void dw_epilogue(const gemm_args &g, const tile_at &at, uint32_t tmem, bool ok)
 {
 	const head_args &h = g.h;
 	const int d = at.m0 + (threadIdx.x & 127);
 	const int v0 = h.v0 + at.n0;
-	const int size = h.bf16 ? 2 : 4;
-	const int64_t first = (int64_t)d * h.lddw + v0;
-	char *out = static_cast<char *>(h.dw) + first * size;
-	const bool vec = ((uintptr_t)out & 31) == 0;
 
 #pragma unroll 1
 	for (int c = 0; c < HEAD_TN && v0 + c < h.v1; c += 32) {
 		float v[32];
 
-		tmem_load(tmem + c, v);
-		if (d >= h.d)
-			continue;
-		if (!vec || v0 + c + 32 > h.v1) {
-#pragma unroll
-			for (int i = 0; i < 32; i++)
-				if (v0 + c + i < h.v1)
-					put(h.dw, first + c + i, v[i], h.bf16, h.add);
-		} else if (h.bf16) {
-#pragma unroll
-			for (int i = 0; i < 32; i += 16) {
-				uint32_t r[8] = { 0, 0, 0, 0, 0, 0, 0, 0 };
-
-				if (h.add)
-					load32(out + (c + i) * 2, r);
-#pragma unroll
-				for (int j = 0; j < 8; j++) {
-					const float2 q = unpack2(r[j]);
-
-					r[j] = bf16_pair(q.x + v[i + 2 * j], q.y + v[i + 2 * j + 1]);
-				}
-				store32(out + (c + i) * 2, r);
-			}
-		} else {
-#pragma unroll
-			for (int i = 0; i < 32; i += 8) {
-				uint32_t r[8] = { 0, 0, 0, 0, 0, 0, 0, 0 };
-
-				if (h.add)
-					load32(out + (c + i) * 4, r);
-#pragma unroll
-				for (int j = 0; j < 8; j++)
-					r[j] = __float_as_uint(__uint_as_float(r[j]) + v[i + j]);
-				store32(out + (c + i) * 4, r);
-			}
-		}
+		tmem_load(tmem + c, ok, v);
+		if (d < h.d)
+			put_row(h.dw, (int64_t)d * h.lddw + v0 + c, v, h.v1 - v0 - c, h.bf16, h.add);
 	}
 }
 
@@ -625,11 +621,11 @@ __device__ __forceinline__ void producer(const gemm_args &g, gemm_smem *s, uint3
 			for (int k = at.k0; k < at.k1; k++, n++) {
 				const uint32_t i = n % HEAD_STAGES;
 
-				if (!mbar_wait(smem_of(&s->empty[i]), (n / HEAD_STAGES & 1) ^ 1, &s->stop, g.h.error)) {
+				if (!mbar_wait(smem_of(&s->empty[i]), (n / HEAD_STAGES & 1) ^ 1, &s->stop)) {
 					if (rank == 0)
 						for (uint32_t j = n < HEAD_STAGES ? 0 : n - HEAD_STAGES; j < n; j++)
 							(void)mbar_wait(smem_of(&s->full[j % HEAD_STAGES]),
-							    j / HEAD_STAGES & 1, NULL, g.h.error);
+							    j / HEAD_STAGES & 1, NULL);
 					else {
 						/* counted elsewhere: no copy is under way for this long */
 						for (const uint64_t end = now_ns() + HEAD_WAIT_NS / 100; now_ns() < end; )
@@ -659,14 +655,14 @@ __device__ __forceinline__ void multiplier(const gemm_args &g, gemm_smem *s, uin
 		const tile_at at = tile_of<KIND>(g, tile, 0);
 		const int steps = (at.k1 - at.k0) * (KIND == DX || KIND == DW ? g.h.terms : 1);
 		const uint32_t acc = s->tmem + (done & 1) * HEAD_TN;
-		bool ok = mbar_wait(smem_of(&s->drained[done & 1]), (done / 2 & 1) ^ 1, &s->stop, g.h.error);
+		bool ok = mbar_wait(smem_of(&s->drained[done & 1]), (done / 2 & 1) ^ 1, &s->stop);
 
 		asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 		for (int k = 0; ok && k < steps; k++, n++) {
 			const uint32_t i = n % HEAD_STAGES;
 			const uint32_t base = ring + i * HEAD_STAGE_BYTES;
 
-			ok = mbar_wait(smem_of(&s->full[i]), n / HEAD_STAGES & 1, &s->stop, g.h.error);
+			ok = mbar_wait(smem_of(&s->full[i]), n / HEAD_STAGES & 1, &s->stop);
 			if (!ok)
 				break;
 			asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -679,7 +675,7 @@ __device__ __forceinline__ void multiplier(const gemm_args &g, gemm_smem *s, uin
 		}
 		if (!ok) {
 			mma_commit(smem_of(&s->quiet));
-			(void)mbar_wait(smem_of(&s->quiet), 0, NULL, g.h.error);
+			(void)mbar_wait(smem_of(&s->quiet), 0, NULL);
 			return;
 		}
 		mma_commit(smem_of(&s->ready[done & 1]));
@@ -702,22 +698,28 @@ __device__ __forceinline__ void drainer(const gemm_args &g, gemm_smem *s, int to
 		if (KIND == DELTA)
 			stage_bias(g.h, g.h.v0 + at.n0, g.h.v1, s->epi.bias[b]);
 		/* the whole warp waits; it keeps step with the other warps even after a give-up, for the barriers' sake */
-		(void)mbar_wait(smem_of(&s->ready[b]), done / 2 & 1, &s->stop, g.h.error);
-		__syncwarp();
+		const bool ok = __all_sync(0xffffffffu, mbar_wait(smem_of(&s->ready[b]), done / 2 & 1, &s->stop));
+
 		asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 		if (KIND == LOSS)
-			loss_epilogue(g, at, acc, s->epi.bias[b]);
+			loss_epilogue(g, at, acc, ok, s->epi.bias[b]);
 		else if (KIND == DELTA)
-			delta_epilogue(g, at, acc, s->epi.bias[b], s->epi.sums[b]);
+			delta_epilogue(g, at, acc, ok, s->epi.bias[b], s->epi.sums[b]);
 		else if (KIND == DX)
-			dx_epilogue(g, at, acc);
+			dx_epilogue(g, at, acc, ok);
 		else
-			dw_epilogue(g, at, acc);
+			dw_epilogue(g, at, acc, ok);
 		asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 		__syncwarp();
 		if ((threadIdx.x & 31) == 0)
 			mbar_arrive_in(smem_in(smem_of(&s->drained[b]), 0));
 	}
+}
+
+/* everything the kernels ahead in the stream have done is visible after this; the next kernel may set itself up */
+__device__ __forceinline__ void dependent(void)
+{
+	asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
 }
 
 __device__ __forceinline__ void cluster_barrier(void)
@@ -760,6 +762,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HEAD_THREADS, 1) pro
 	__syncthreads();
 	cluster_barrier();
 	asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+	dependent();
 	if (warp == 0) {
 		if ((threadIdx.x & 31) == 0)
 			producer<KIND>(g, &s, ring, total, rank, pair, pairs);
@@ -798,6 +801,7 @@ __global__ void __launch_bounds__(1024) join_kernel(const head_args h, int tiles
 	float top = -INFINITY;
 	float sum = 0.0f;
 
+	dependent();
 	if (t < h.tokens) {
 #pragma unroll 4
 		for (int k = w; k < tiles; k += 32)
@@ -813,11 +817,11 @@ __global__ void __launch_bounds__(1024) join_kernel(const head_args h, int tiles
 	for (int k = 16; k > 0; k >>= 1)
 		join(top, sum, make_float2(__shfl_down_sync(0xffffffffu, top, k), __shfl_down_sync(0xffffffffu, sum, k)));
 	if (lane == 0 && t < h.tokens) {
-		const float lse = *h.error ? NAN : top + logf(sum);
+		const float lse = top + logf(sum);
 		const int y = h.target[t];
 
 		h.lse[t] = lse;
-		h.nll[t] = y < 0 ? (*h.error ? NAN : 0.0f) : y >= h.vocab ? NAN : lse - h.hit[t];
+		h.nll[t] = y < 0 ? 0.0f : y >= h.vocab ? NAN : lse - h.hit[t];
 	}
 }
 
@@ -830,41 +834,43 @@ __device__ __forceinline__ float row_factor(const head_args &h, int t)
 }
 
 /*
-** Rows of bf16 to a 16-byte grid, one block per row.  With ROWS also their factors, and zeros for the rows
+** Rows of bf16 to a 16-byte grid, 16 bytes a thread.  With ROWS also their factors, and zeros for the rows
 ** without a gradient, so that whatever they hold meets a delta of 0 as 0.
 */
 template <bool ROWS>
-__global__ void __launch_bounds__(128) pack_kernel(const head_args h, __nv_bfloat16 *to, int64_t ldt, const __nv_bfloat16 *from,
+__global__ void __launch_bounds__(256) pack_kernel(const head_args h, __nv_bfloat16 *to, int ldt, const __nv_bfloat16 *from,
 	int64_t ldf, int rows, int cols)
 {
-	for (int r = blockIdx.x; r < rows; r += gridDim.x) {
-		const float f = ROWS ? row_factor(h, r) : 1.0f;
-		const __nv_bfloat16 *src = from + (int64_t)r * ldf;
-		__nv_bfloat16 *dst = to + (int64_t)r * ldt;
-		const bool on = f != 0.0f;
+	const int per = ldt / 8;
+	const int64_t total = (int64_t)rows * per;
 
-		if (ROWS && threadIdx.x == 0)
+	dependent();
+	for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+		const int r = (int)(i / per);
+		const int c = (int)(i - (int64_t)r * per) * 8;
+		const float f = ROWS ? row_factor(h, r) : 1.0f;
+		const __nv_bfloat16 *src = from + (int64_t)r * ldf + c;
+		uint32_t q[4] = { 0, 0, 0, 0 };
+
+		if (ROWS && c == 0)
 			h.row[r] = f;
-		if (((uintptr_t)src & 15) == 0)
-			for (int i = threadIdx.x * 8; i < cols; i += 128 * 8) {
-				if (i + 8 <= cols)
-					*reinterpret_cast<uint4 *>(dst + i) = on ? *reinterpret_cast<const uint4 *>(src + i)
-					    : make_uint4(0, 0, 0, 0);
-				else
-					for (int j = i; j < cols; j++)
-						dst[j] = on ? src[j] : __float2bfloat16_rn(0.0f);
-			}
-		else
-			for (int i = threadIdx.x; i < cols; i += 128)
-				dst[i] = on ? src[i] : __float2bfloat16_rn(0.0f);
+		if (f != 0.0f) {
+			if (c + 8 <= cols && ((uintptr_t)src & 15) == 0)
+				*reinterpret_cast<uint4 *>(q) = *reinterpret_cast<const uint4 *>(src);
+			else
+#pragma unroll
+				for (int j = 0; j < 8; j++)
+					if (c + j < cols)
+						q[j / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(src)[j] << (j % 2 * 16);
+		}
+		*reinterpret_cast<uint4 *>(to + (int64_t)r * ldt + c) = make_uint4(q[0], q[1], q[2], q[3]);
 	}
 }
 
 /* the parts of dx added up in order; a block takes a row at a time */
 __global__ void __launch_bounds__(128) finish_dx_kernel(const head_args h)
 {
-	const bool bad = *h.error != 0;
-
+	dependent();
 	for (int t = blockIdx.x; t < h.tokens; t += gridDim.x) {
 		const int size = h.bf16 ? 2 : 4;
 		char *out = static_cast<char *>(h.dx) + (int64_t)t * h.lddx * size;
@@ -880,8 +886,6 @@ __global__ void __launch_bounds__(128) finish_dx_kernel(const head_args h)
 				v.z += q.z;
 				v.w += q.w;
 			}
-			if (bad)
-				v = make_float4(NAN, NAN, NAN, NAN);
 			if (d + 4 <= h.d && ((uintptr_t)out & 15) == 0) {
 				if (h.bf16)
 					*reinterpret_cast<uint2 *>(out + d * 2) = make_uint2(bf16_pair(v.x, v.y), bf16_pair(v.z, v.w));
@@ -904,13 +908,14 @@ __global__ void __launch_bounds__(256) finish_db_kernel(const head_args h, int t
 	const int v = blockIdx.x * blockDim.x + threadIdx.x;
 	double s = 0.0;
 
+	dependent();
 	if (v >= h.vocab)
 		return;
 	for (int k = 0; k < tiles; k++)
 		s += (double)h.dbp[(int64_t)k * h.vocab + v];
 	if (h.add)
 		s += h.bf16 ? (double)to_f(static_cast<__nv_bfloat16 *>(h.db)[v]) : (double)static_cast<float *>(h.db)[v];
-	put(h.db, v, *h.error ? NAN : (float)s, h.bf16, 0);
+	put(h.db, v, (float)s, h.bf16, 0);
 }
 
 /* ---- host --------------------------------------------------------------------------------------- */
@@ -938,6 +943,7 @@ struct head_plan {
 	int	piece;
 	int	terms;
 	int	splits;
+	int	parts;		/* dx is added up in fp32 in the workspace */
 	int	ldd;
 };
 
@@ -1010,7 +1016,6 @@ head_plan plan_of(const anni_head_call *c, int grad)
 	const int64_t t = std::max<int64_t>(c->tokens, 1);
 
 	memset(&p, 0, sizeof(p));
-	p.bytes = 256;		/* the error word */
 	p.copy_x = grad || (c->ldx & 7) || ((uintptr_t)c->x & 15);
 	p.copy_w = (c->ldw & 7) || ((uintptr_t)c->w & 15);
 	p.ldx = up(c->d_model, 8);
@@ -1023,14 +1028,16 @@ head_plan plan_of(const anni_head_call *c, int grad)
 		return p;
 	}
 	p.terms = c->grad_dtype == ANNI_DT_BF16 ? 1 : HEAD_TERMS;
-	p.piece = (int)std::min<int64_t>(up(c->vocab, 256),
-	    std::max<int64_t>(256, (int64_t)(HEAD_PIECE_BYTES / (size_t)(t * 2 * p.terms)) / 256 * 256));
+	/* as many columns of delta as HEAD_PIECE_BYTES hold, then pieces of about the same size */
+	p.piece = (int)std::max<int64_t>(HEAD_TN, (int64_t)(HEAD_PIECE_BYTES / (size_t)(t * 2 * p.terms)) / HEAD_TN * HEAD_TN);
+	p.piece = (int)up((c->vocab + (c->vocab + p.piece - 1) / p.piece - 1) / ((c->vocab + p.piece - 1) / p.piece), HEAD_TN);
 	p.row = take(&p.bytes, t * 4);
 	p.delta = take(&p.bytes, (int64_t)p.piece * t * 2 * p.terms);
-	p.ldd = (int)up(c->d_model, 4);
+	p.ldd = (int)up(c->d_model, 8);
 	p.splits = split_dx(up(t, HEAD_TM) / HEAD_TM * (up(c->d_model, HEAD_TN) / HEAD_TN),
 	    up(std::min(p.piece, c->vocab), HEAD_TK) / HEAD_TK);
-	p.dxp = take(&p.bytes, c->dx ? p.splits * t * p.ldd * 4 : 0);
+	p.parts = c->dx && (p.splits > 1 || p.piece < c->vocab);
+	p.dxp = take(&p.bytes, p.parts ? p.splits * t * p.ldd * 4 : 0);
 	p.dbp = take(&p.bytes, c->dbias ? up(t, HEAD_HALF) / HEAD_HALF * c->vocab * 4 : 0);
 	return p;
 }
@@ -1060,7 +1067,7 @@ head_args args_of(const anni_head_call *c, const head_plan &p)
 	h.delta = reinterpret_cast<__nv_bfloat16 *>(ws + p.delta);
 	h.terms = p.terms;
 	h.ldp = p.piece;
-	h.dxp = reinterpret_cast<float *>(ws + p.dxp);
+	h.dxp = p.parts ? reinterpret_cast<float *>(ws + p.dxp) : NULL;
 	h.ldd = p.ldd;
 	h.splits = p.splits;
 	h.dbp = reinterpret_cast<float *>(ws + p.dbp);
@@ -1071,7 +1078,6 @@ head_args args_of(const anni_head_call *c, const head_plan &p)
 	h.db = c->dbias;
 	h.bf16 = c->grad_dtype == ANNI_DT_BF16;
 	h.add = (c->flags & ANNI_HEAD_ACCUMULATE) != 0;
-	h.error = reinterpret_cast<int *>(ws);
 	return h;
 }
 
@@ -1080,10 +1086,36 @@ unsigned tiles(int64_t n, int64_t of)
 	return (unsigned)((n + of - 1) / of);
 }
 
-int launched(void)
+/*
+** Launches a kernel that may start before the one ahead of it in the stream has ended: its blocks set themselves
+** up meanwhile and wait (dependent()) before they touch memory.
+*/
+template <typename... P, typename... A>
+int launch(void (*kernel)(P...), int64_t grid, int threads, int smem, cudaStream_t st, A... args)
 {
+	cudaLaunchConfig_t cfg = {};
+	cudaLaunchAttribute early;
+
+	early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+	early.val.programmaticStreamSerializationAllowed = 1;
+	cfg.gridDim = dim3((unsigned)grid);
+	cfg.blockDim = dim3((unsigned)threads);
+	cfg.dynamicSmemBytes = (size_t)smem;
+	cfg.stream = st;
+	cfg.attrs = &early;
+	cfg.numAttrs = 1;
+	if (cudaLaunchKernelEx(&cfg, kernel, P(args)...) != cudaSuccess) {
+		(void)cudaGetLastError();
+		return ANNI_E_CUDA;
+	}
 	anni_count_launch();
-	return cudaGetLastError() == cudaSuccess ? ANNI_OK : ANNI_E_CUDA;
+	return ANNI_OK;
+}
+
+/* blocks of 256 threads with 16 bytes each */
+int64_t blocks(int64_t rows, int64_t ld)
+{
+	return std::min<int64_t>((rows * ld / 8 + 255) / 256, 16 * 2 * HEAD_PAIRS);
 }
 
 typedef CUresult (*encode_fn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
@@ -1120,6 +1152,35 @@ int tensor_map(CUtensorMap *m, const void *base, int64_t cols, int64_t rows, int
 	    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? ANNI_OK : ANNI_E_CUDA;
 }
 
+/*
+** Number of SMs of the current device, and the kernel's shared memory allowed on it; asked for once per device
+** (devices beyond the table are asked every time).
+*/
+#define HEAD_DEVICES	16
+std::atomic<int> known[4][HEAD_DEVICES];
+
+template <typename K>
+int ready(K kernel, int smem, int *sms, std::atomic<int> (*seen)[HEAD_DEVICES])
+{
+	int dev = 0;
+	int n = 0;
+
+	if (cudaGetDevice(&dev) != cudaSuccess)
+		return ANNI_E_CUDA;
+	n = dev < HEAD_DEVICES ? (*seen)[dev].load(std::memory_order_relaxed) : 0;
+	if (n == 0) {
+		if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess
+		    || cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+			(void)cudaGetLastError();
+			return ANNI_E_CUDA;
+		}
+		if (dev < HEAD_DEVICES)
+			(*seen)[dev].store(n, std::memory_order_relaxed);
+	}
+	*sms = n;
+	return ANNI_OK;
+}
+
 /* the product of one kind over the piece h.v0 .. h.v1 of the vocabulary */
 template <int KIND>
 int product(const head_args &h, cudaStream_t st)
@@ -1127,7 +1188,6 @@ int product(const head_args &h, cudaStream_t st)
 	const int smem = HEAD_STAGES * HEAD_STAGE_BYTES + 1024;
 	const int width = h.v1 - h.v0;
 	gemm_args g;
-	int dev;
 	int sms;
 	int rc;
 
@@ -1153,14 +1213,11 @@ int product(const head_args &h, cudaStream_t st)
 	}
 	if (rc != ANNI_OK)
 		return rc;
-	if (cudaGetDevice(&dev) != cudaSuccess
-	    || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess
-	    || cudaFuncSetAttribute(product_kernel<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
-		(void)cudaGetLastError();
-		return ANNI_E_CUDA;
-	}
-	product_kernel<KIND><<<2 * std::min(sms / 2, g.m_tiles * g.n_tiles * (KIND == DX ? h.splits : 1)), HEAD_THREADS, smem, st>>>(g);
-	return launched();
+	rc = ready(product_kernel<KIND>, smem, &sms, &known[KIND]);
+	if (rc != ANNI_OK)
+		return rc;
+	return launch(product_kernel<KIND>, 2 * std::min(sms / 2, g.m_tiles * g.n_tiles * (KIND == DX ? h.splits : 1)), HEAD_THREADS,
+	    smem, st, g);
 }
 
 /* the copies that the plan asks for; x's with the factors of the rows when gradients follow */
@@ -1170,20 +1227,15 @@ int pack(const anni_head_call *c, const head_plan &p, const head_args &h, bool g
 	__nv_bfloat16 *w = const_cast<__nv_bfloat16 *>(h.w);
 	int rc = ANNI_OK;
 
-	if (grad || p.copy_x) {
-		const __nv_bfloat16 *from = static_cast<const __nv_bfloat16 *>(c->x);
-
-		if (grad)
-			pack_kernel<true><<<std::min(h.tokens, 8192), 128, 0, st>>>(h, x, h.ldx, from, c->ldx, h.tokens, h.d);
-		else
-			pack_kernel<false><<<std::min(h.tokens, 8192), 128, 0, st>>>(h, x, h.ldx, from, c->ldx, h.tokens, h.d);
-		rc = launched();
-	}
-	if (rc == ANNI_OK && p.copy_w) {
-		pack_kernel<false><<<std::min(h.d, 8192), 128, 0, st>>>(h, w, h.ldw, static_cast<const __nv_bfloat16 *>(c->w), c->ldw,
-		    h.d, h.vocab);
-		rc = launched();
-	}
+	if (grad)
+		rc = launch(pack_kernel<true>, blocks(h.tokens, h.ldx), 256, 0, st, h, x, (int)h.ldx,
+		    static_cast<const __nv_bfloat16 *>(c->x), c->ldx, h.tokens, h.d);
+	else if (p.copy_x)
+		rc = launch(pack_kernel<false>, blocks(h.tokens, h.ldx), 256, 0, st, h, x, (int)h.ldx,
+		    static_cast<const __nv_bfloat16 *>(c->x), c->ldx, h.tokens, h.d);
+	if (rc == ANNI_OK && p.copy_w)
+		rc = launch(pack_kernel<false>, blocks(h.d, h.ldw), 256, 0, st, h, w, (int)h.ldw,
+		    static_cast<const __nv_bfloat16 *>(c->w), c->ldw, h.d, h.vocab);
 	return rc;
 }
 
@@ -1213,16 +1265,12 @@ extern "C" int anni_head_loss(const anni_head_call *c, void *stream)
 	if (rc != ANNI_OK)
 		return rc;
 	h = args_of(c, p);
-	if (cudaMemsetAsync(h.error, 0, 256, st) != cudaSuccess)
-		return ANNI_E_CUDA;
 	rc = pack(c, p, h, false, st);
 	h.v1 = h.vocab;
 	if (rc == ANNI_OK)
 		rc = product<LOSS>(h, st);
-	if (rc == ANNI_OK) {
-		join_kernel<<<tiles(h.tokens, 32), 1024, 0, st>>>(h, (int)tiles(h.vocab, HEAD_TN));
-		rc = launched();
-	}
+	if (rc == ANNI_OK)
+		rc = launch(join_kernel, tiles(h.tokens, 32), 1024, 0, st, h, (int)tiles(h.vocab, HEAD_TN));
 	return rc;
 }
 
@@ -1256,8 +1304,6 @@ extern "C" int anni_head_loss_grad(const anni_head_call *c, void *stream)
 	if (rc != ANNI_OK)
 		return rc;
 	h = args_of(c, p);
-	if (cudaMemsetAsync(h.error, 0, 256, st) != cudaSuccess)
-		return ANNI_E_CUDA;
 	rc = pack(c, p, h, true, st);
 	for (h.v0 = 0; rc == ANNI_OK && h.v0 < h.vocab; h.v0 = h.v1) {
 		h.v1 = std::min(h.vocab, h.v0 + p.piece);
@@ -1267,25 +1313,9 @@ extern "C" int anni_head_loss_grad(const anni_head_call *c, void *stream)
 		if (rc == ANNI_OK && h.dw)
 			rc = product<DW>(h, st);
 	}
-	if (rc == ANNI_OK && h.dx) {
-		finish_dx_kernel<<<std::min(h.tokens, 16384), 128, 0, st>>>(h);
-		rc = launched();
-	}
-	if (rc == ANNI_OK && h.db) {
-		finish_db_kernel<<<tiles(h.vocab, 256), 256, 0, st>>>(h, (int)tiles(h.tokens, HEAD_HALF));
-		rc = launched();
-	}
+	if (rc == ANNI_OK && h.dxp)
+		rc = launch(finish_dx_kernel, std::min(h.tokens, 16384), 128, 0, st, h);
+	if (rc == ANNI_OK && h.db)
+		rc = launch(finish_db_kernel, tiles(h.vocab, 256), 256, 0, st, h, (int)tiles(h.tokens, HEAD_HALF));
 	return rc;
-}
-
-extern "C" int anni_head_status(const anni_head_call *c, void *stream)
-{
-	int error = 0;
-
-	if (!c || !c->workspace)
-		return ANNI_E_ARG;
-	if (cudaStreamSynchronize((cudaStream_t)stream) != cudaSuccess
-	    || cudaMemcpy(&error, c->workspace, sizeof(error), cudaMemcpyDeviceToHost) != cudaSuccess)
-		return ANNI_E_CUDA;
-	return error;
 }

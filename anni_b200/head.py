@@ -3,6 +3,7 @@
 ``head_loss`` and ``head_loss_grad`` take torch tensors, allocate their workspace from torch for the length of
 the call and run on the current stream; nothing is kept between calls.
 """
+import contextlib
 import ctypes as C
 
 import torch
@@ -35,7 +36,7 @@ def lib():
         P = C.POINTER(Call)
         L.anni_head_workspace.restype = C.c_int
         L.anni_head_workspace.argtypes = [P, C.c_int, C.POINTER(C.c_size_t)]
-        for f in (L.anni_head_loss, L.anni_head_loss_grad, L.anni_head_status):
+        for f in (L.anni_head_loss, L.anni_head_loss_grad):
             f.restype = C.c_int
             f.argtypes = [P, C.c_void_p]
         _L = L
@@ -72,27 +73,34 @@ def _call(x, w, target, bias):
     return c
 
 
-def _run(name, c, grad, device, stream):
+def _here(device, stream):
+    """A context in which `device` and `stream` are current; nothing to do where they are already."""
+    if stream is None and device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    both = contextlib.ExitStack()
+    both.enter_context(torch.cuda.device(device))
+    both.enter_context(torch.cuda.stream(stream))       # None: no change
+    return both
+
+
+def _run(name, c, grad, device):
     L = lib()
-    s = torch.cuda.current_stream(device) if stream is None else stream
     need = C.c_size_t()
-    check("anni_head_workspace", L.anni_head_workspace(C.byref(c), grad, C.byref(need)))
-    with torch.cuda.device(device), torch.cuda.stream(s):
-        # the allocator hands the block to later work of this stream only: no other call can hold it meanwhile
-        ws = torch.empty(need.value, dtype=torch.uint8, device=device)
-        c.workspace, c.workspace_bytes = ws.data_ptr(), need.value
-        check(name, getattr(L, name)(C.byref(c), s.cuda_stream))
+    check("anni_head_workspace", L.anni_head_workspace(c, grad, need))
+    # the allocator hands the block to later work of this stream only: no other call can hold it meanwhile
+    ws = torch.empty(need.value, dtype=torch.uint8, device=device)
+    c.workspace, c.workspace_bytes = ws.data_ptr(), need.value
+    check(name, getattr(L, name)(c, torch.cuda.current_stream(device).cuda_stream))
 
 
 def head_loss(x, w, target, *, bias=None, stream=None):
     """Rows of (nll, lse): x bf16 (tokens, d_model), w bf16 (d_model, vocab), target int32 (tokens), bias fp32
     (vocab) or None.  A target below 0 is ignored (nll 0), one beyond the vocabulary gives NaN."""
     c = _call(x, w, target, bias)
-    s = torch.cuda.current_stream(x.device) if stream is None else stream
-    with torch.cuda.stream(s):
-        nll, lse = torch.empty(2, c.tokens, dtype=torch.float32, device=x.device)
-    c.nll, c.lse = nll.data_ptr(), lse.data_ptr()
-    _run("anni_head_loss", c, 0, x.device, s)
+    with _here(x.device, stream):
+        nll, lse = torch.empty(2, c.tokens, dtype=torch.float32, device=x.device).unbind(0)
+        c.nll, c.lse = nll.data_ptr(), lse.data_ptr()
+        _run("anni_head_loss", c, 0, x.device)
     return nll, lse
 
 
@@ -116,4 +124,5 @@ def head_loss_grad(x, w, target, lse, *, bias=None, weight=None, grad_scale=1.0,
         c.dw, c.lddw = _rows("dw", dw, c.d_model, c.vocab, kind, x.device)
     if dbias is not None:
         c.dbias = _flat("dbias", dbias, c.vocab, kind, x.device)
-    _run("anni_head_loss_grad", c, 1, x.device, stream)
+    with _here(x.device, stream):
+        _run("anni_head_loss_grad", c, 1, x.device)

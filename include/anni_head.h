@@ -23,6 +23,9 @@
 ** it is carried as three bf16 terms (24 bits), so dx and dw are good to fp32.  dbias is summed in fp32
 ** from the unrounded delta.  Sums run in a fixed order: the same inputs give the same bits.
 **
+** Waits inside the kernels are bounded: a block that gives up (two seconds without progress) fills what it
+** has not computed with NaN, which shows in nll, dx, dw and dbias.
+**
 ** Nothing is allocated and nothing is kept: all working memory is the caller's, and calls that use
 ** different workspaces are independent.  Work runs on the current device, which must hold the buffers.
 */
@@ -86,11 +89,6 @@ int	anni_head_workspace(const anni_head_call *c, int grad, size_t *bytes);
 int	anni_head_loss(const anni_head_call *c, void *stream);
 /* dx, dw, dbias from lse, which an anni_head_loss on the same x, w, bias has written. */
 int	anni_head_loss_grad(const anni_head_call *c, void *stream);
-/*
-** Waits for `stream` and says whether a bounded wait inside the last call on this workspace gave up:
-** ANNI_OK or ANNI_E_BARRIER_TIMEOUT (its outputs are NaN then).
-*/
-int	anni_head_status(const anni_head_call *c, void *stream);
 
 #ifdef __cplusplus
 }

@@ -420,7 +420,7 @@ def test_limits(kw):
 def test_null_and_empty_calls():
     L = head.lib()
     n = C.c_size_t()
-    assert L.anni_head_loss(None, None) == L.anni_head_loss_grad(None, None) == L.anni_head_status(None, None) == capi.E_ARG
+    assert L.anni_head_loss(None, None) == L.anni_head_loss_grad(None, None) == capi.E_ARG
     assert L.anni_head_workspace(None, 0, C.byref(n)) == capi.E_ARG and L.anni_head_workspace(C.byref(_c()), 0, None) == capi.E_ARG
     assert L.anni_head_loss(C.byref(_c(tokens=0, x=None, workspace=None)), None) == capi.OK
     assert L.anni_head_loss_grad(C.byref(_c(dx=None, dw=None, dbias=None, workspace=None)), None) == capi.OK
@@ -438,4 +438,4 @@ def test_workspace_is_bounded():
 def test_every_declared_symbol_is_exported():
     from test_abi_cpu import _declared_symbols
     names = _declared_symbols("anni_head.h")
-    assert len(names) >= 4 and not [k for k in names if not hasattr(head.lib(), k)]
+    assert len(names) == 3 and not [k for k in names if not hasattr(head.lib(), k)]
