@@ -13,10 +13,15 @@
 ** Two blocks (a cluster on two neighbouring SMs) work on a 256 x 256 tile: each keeps 128 rows of the result
 ** and loads its 128 rows of the one operand and 128 of the other by TMA into a ring of HEAD_STAGES stages; one
 ** thread of the first block issues tcgen05.mma for both SMs, which read half of the second operand from each
-** other's shared memory, into one of two accumulators in tensor memory, while four warps of each block empty
+** other's shared memory, into one of two accumulators in tensor memory, while eight warps of each block empty
 ** the other one.  An operand whose rows run along the summed dimension ("K-major") is loaded as one box
 ** of 64 k x rows, one whose rows run along the result ("MN-major") as boxes of 64 mn x 64 k, so nothing is
 ** transposed in memory.  Lengths that are no multiple of a tile end in zeros that TMA fills in.
+**
+** The tensor cores cut their running sums off instead of rounding them: over K terms a result drifts towards zero
+** by about 3e-9 K of its size (measured: log-sum-exp of 1001 terms low by 3.6e-6, an fp32 gradient over 8192
+** rows off by 2.5e-5).  Where that matters a sum is taken in runs: the warps that empty an accumulator add it to sums in
+** their registers, rounded, and the next run starts from zero.
 */
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -39,7 +44,10 @@
 #define HEAD_B_BYTES	(HEAD_HALF * HEAD_TK * 2)
 #define HEAD_STAGE_BYTES (HEAD_A_BYTES + HEAD_B_BYTES)
 #define HEAD_MN_BYTES	(64 * HEAD_TK * 2)	/* one MN-major box */
-#define HEAD_THREADS	256
+#define HEAD_EPI	256	/* threads that empty accumulators: 128 rows x 2 halves of the columns */
+#define HEAD_THREADS	(128 + HEAD_EPI)
+#define HEAD_RUN	8	/* stages in one run of a sum: 512 terms of a logit, */
+#define HEAD_RUN_F32	4	/* 256 of an fp32 gradient */
 #define HEAD_PAIRS	74	/* pairs of SMs that the work is cut for; any number of them runs it */
 #define HEAD_PIECE_BYTES ((size_t)256 << 20)	/* of delta in the workspace */
 #define HEAD_TERMS	3	/* bf16 terms of delta for fp32 gradients */
@@ -91,6 +99,7 @@ struct gemm_args {
 	int		m_tiles;
 	int		n_tiles;
 	int		k_blocks;	/* of one term */
+	int		run;		/* ... of them that one accumulator adds up */
 };
 
 /* ---- PTX ------------------------------------------------------------------------------------------ */
@@ -210,23 +219,25 @@ __device__ __forceinline__ void mma_commit(uint32_t bar)
 	    :: "r"(bar), "h"((uint16_t)3) : "memory");
 }
 
-/* 32 columns of this warp's 32 lanes of tensor memory: lane l gets row l (ok false: NaN) */
-__device__ __forceinline__ void tmem_load(uint32_t addr, bool ok, float (&v)[32])
+/* 32 columns of this warp's 32 lanes of tensor memory: lane l gets row l; valid after tmem_wait() */
+__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32])
 {
-	uint32_t r[32];
-
-	__syncwarp();		/* rows that do not exist go other ways between two loads */
 	asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
 	    "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
 	    "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-	    : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-	    "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-	    "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-	    "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]) : "r"(addr));
-	asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-	for (int i = 0; i < 32; i++)
-		v[i] = ok ? __uint_as_float(r[i]) : NAN;
+	    : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+	    "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
+	    "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+	    "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31]) : "r"(addr));
+}
+
+/* the values of the loads before are there: nothing that uses them may be moved ahead of it */
+__device__ __forceinline__ void tmem_wait(float (&v)[32])
+{
+	asm volatile("tcgen05.wait::ld.sync.aligned;" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]),
+	    "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]),
+	    "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]),
+	    "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31]) :: "memory");
 }
 
 __device__ __forceinline__ float exp2_approx(float x)
@@ -336,23 +347,41 @@ __device__ __forceinline__ void load_stage(const gemm_args &g, const tile_at &t,
 	}
 }
 
-/* ---- epilogues: one warp's 32 rows of a tile, 32 columns at a time -------------------------------- */
+/* ---- epilogues: a thread has 128 columns of one row, as four times 32 --------------------------------- */
 
 struct epi_smem {
 	float	bias[2][HEAD_TN];	/* of two tiles; -inf beyond the vocabulary */
-	float	sums[2][4][HEAD_TN];	/* delta: column sums of each warp's rows */
+	float	sums[2][4][HEAD_TN];	/* delta: column sums of each quarter of the rows */
+	float2	half[2][HEAD_HALF];	/* loss: maximum and sum of the second half of the columns */
 };
 
 __device__ __forceinline__ void epi_barrier(void)
 {
-	asm volatile("bar.sync 1, 128;" ::: "memory");
+	asm volatile("bar.sync 1, 256;" ::: "memory");
 }
 
-/* biases of the tile's columns, staged by the four epilogue warps */
+/* row of the block's 128, first column of the tile's 256, and number among the epilogue's threads */
+__device__ __forceinline__ int epi_row(void)
+{
+	return threadIdx.x & (HEAD_HALF - 1);
+}
+
+__device__ __forceinline__ int epi_thread(void)
+{
+	return threadIdx.x - 128;
+}
+
+__device__ __forceinline__ int epi_col(void)
+{
+	return epi_thread() / HEAD_HALF * 128;
+}
+
+/* biases of the tile's columns */
 __device__ __forceinline__ void stage_bias(const head_args &h, int v0, int end, float *to)
 {
-	for (int i = threadIdx.x & 127; i < HEAD_TN; i += 128)
-		to[i] = v0 + i >= end ? -INFINITY : h.bias ? __ldg(h.bias + v0 + i) : 0.0f;
+	const int i = epi_thread();
+
+	to[i] = v0 + i >= end ? -INFINITY : h.bias ? __ldg(h.bias + v0 + i) : 0.0f;
 	epi_barrier();
 }
 
@@ -377,35 +406,36 @@ __device__ __forceinline__ float column_sums(float (&v)[32])
 }
 
 /* one pass over the columns with a running maximum and a sum that follows it */
-__device__ __forceinline__ void loss_epilogue(const gemm_args &g, const tile_at &at, uint32_t tmem, bool ok, const float *bias)
+__device__ __forceinline__ void loss_epilogue(const gemm_args &g, const tile_at &at, float (&acc)[4][32], const float *bias,
+	float2 *half)
 {
 	const head_args &h = g.h;
-	const int t = at.m0 + (threadIdx.x & 127);
+	const int t = at.m0 + epi_row();
 	const int y = t < h.tokens ? h.target[t] : -1;
-	const int rel = y >= at.n0 && y < h.vocab && y < at.n0 + HEAD_TN ? y - at.n0 : -1;
+	const int c0 = epi_col();
+	const int rel = y >= at.n0 + c0 && y < h.vocab && y < at.n0 + c0 + 128 ? y - at.n0 - c0 : -1;
 	float top = -INFINITY;
 	float sum = 0.0f;
 
-#pragma unroll 1
-	for (int c = 0; c < HEAD_TN; c += 32) {
-		float v[32];
+#pragma unroll
+	for (int c = 0; c < 4; c++) {
+		float (&v)[32] = acc[c];
 		float high;
 		float base;
 
-		tmem_load(tmem + c, ok, v);
 #pragma unroll
 		for (int i = 0; i < 32; i += 4) {
-			const float4 b = *reinterpret_cast<const float4 *>(bias + c + i);
+			const float4 b = *reinterpret_cast<const float4 *>(bias + c0 + c * 32 + i);
 
 			v[i] += b.x;
 			v[i + 1] += b.y;
 			v[i + 2] += b.z;
 			v[i + 3] += b.w;
 		}
-		if (__any_sync(0xffffffffu, rel >= c && rel < c + 32)) {	/* one in vocab / 32 chunks of a row */
+		if (__any_sync(0xffffffffu, rel >= c * 32 && rel < c * 32 + 32)) {	/* one in vocab / 32 chunks of a row */
 #pragma unroll
 			for (int i = 0; i < 32; i++)
-				if (rel == c + i)
+				if (rel == c * 32 + i)
 					h.hit[t] = v[i];
 		}
 		high = v[0];
@@ -420,79 +450,97 @@ __device__ __forceinline__ void loss_epilogue(const gemm_args &g, const tile_at 
 		for (int i = 0; i < 32; i++)
 			sum += exp2_approx((v[i] - base) * LOG2E);
 	}
-	if (t < h.tokens)
-		h.part[(int64_t)(at.n0 / HEAD_TN) * h.tokens + t] = make_float2(top, sum);
+	if (c0)
+		half[epi_row()] = make_float2(top, sum);
+	epi_barrier();
+	if (!c0 && t < h.tokens) {
+		const float2 p = half[epi_row()];
+		const float high = fmaxf(top, p.x);
+		const float base = high == -INFINITY ? 0.0f : high;
+
+		sum = sum * exp2_approx((top - base) * LOG2E) + p.y * exp2_approx((p.x - base) * LOG2E);
+		h.part[(int64_t)(at.n0 / HEAD_TN) * h.tokens + t] = make_float2(high, sum);
+	}
 }
 
-__device__ __forceinline__ void delta_epilogue(const gemm_args &g, const tile_at &at, uint32_t tmem, bool ok, const float *bias,
+__device__ __forceinline__ void delta_epilogue(const gemm_args &g, const tile_at &at, float (&acc)[4][32], const float *bias,
 	float (*sums)[HEAD_TN])
 {
 	const head_args &h = g.h;
 	const int lane = threadIdx.x & 31;
-	const int wq = threadIdx.x >> 5 & 3;
-	const int t = at.m0 + (threadIdx.x & 127);
+	const int c0 = epi_col();
+	const int t = at.m0 + epi_row();
 	const float f = t < h.tokens ? h.row[t] : 0.0f;
 	const float lse = f != 0.0f ? h.lse[t] : 0.0f;
-	const int y = f != 0.0f ? h.target[t] - h.v0 - at.n0 : -1;
-	__nv_bfloat16 *out = h.delta + (int64_t)t * h.ldp + at.n0;
+	const int y = f != 0.0f ? h.target[t] - h.v0 - at.n0 - c0 : -1;
+	__nv_bfloat16 *out = h.delta + (int64_t)t * h.ldp + at.n0 + c0;
 
-#pragma unroll 1
-	for (int c = 0; c < HEAD_TN; c += 32) {
-		float v[32];
+#pragma unroll
+	for (int c = 0; c < 4; c++) {
+		float (&v)[32] = acc[c];
 
-		tmem_load(tmem + c, ok, v);
 #pragma unroll
 		for (int i = 0; i < 32; i += 4) {
-			const float4 b = *reinterpret_cast<const float4 *>(bias + c + i);
+			const float4 b = *reinterpret_cast<const float4 *>(bias + c0 + c * 32 + i);
 
 			v[i] = exp2_approx((v[i] + b.x - lse) * LOG2E);
 			v[i + 1] = exp2_approx((v[i + 1] + b.y - lse) * LOG2E);
 			v[i + 2] = exp2_approx((v[i + 2] + b.z - lse) * LOG2E);
 			v[i + 3] = exp2_approx((v[i + 3] + b.w - lse) * LOG2E);
 		}
-		if (__any_sync(0xffffffffu, y >= c && y < c + 32)) {
+		if (__any_sync(0xffffffffu, y >= c * 32 && y < c * 32 + 32)) {
 #pragma unroll
 			for (int i = 0; i < 32; i++)
-				if (y == c + i)
+				if (y == c * 32 + i)
 					v[i] -= 1.0f;
 		}
 #pragma unroll
 		for (int i = 0; i < 32; i++)
 			v[i] = f != 0.0f ? v[i] * f : 0.0f;
 		if (t < h.tokens) {
-			float rest[32];
+			__nv_bfloat16 *q = out + c * 32;
 
-#pragma unroll
-			for (int i = 0; i < 32; i++)
-				rest[i] = v[i];
-			/* the largest term last: the products add the small ones up first */
-			for (int k = h.terms - 1; k >= 0; k--) {
-				__nv_bfloat16 *q = out + (int64_t)k * h.tokens * h.ldp + c;
-
+			for (int n = 1; n < h.terms; n++) {	/* fp32 gradients: first the terms that correct the largest */
 #pragma unroll
 				for (int i = 0; i < 32; i += 16) {
 					uint32_t r[8];
 
 #pragma unroll
-					for (int j = 0; j < 8; j++)
-						r[j] = bf16_pair(rest[i + 2 * j], rest[i + 2 * j + 1]);
-					store32(q + i, r);
+					for (int j = 0; j < 8; j++) {
+						float lo = v[i + 2 * j];
+						float hi = v[i + 2 * j + 1];
+
+#pragma unroll 1
+						for (int k = 0; k < n; k++) {
+							lo -= to_f(__float2bfloat16_rn(lo));
+							hi -= to_f(__float2bfloat16_rn(hi));
+						}
+						r[j] = bf16_pair(lo, hi);
+					}
+					store32(q + (int64_t)n * h.tokens * h.ldp + i, r);
 				}
-				if (k > 0)
+			}
 #pragma unroll
-					for (int i = 0; i < 32; i++)
-						rest[i] -= to_f(__float2bfloat16_rn(rest[i]));
+			for (int i = 0; i < 32; i += 16) {
+				uint32_t r[8];
+
+#pragma unroll
+				for (int j = 0; j < 8; j++)
+					r[j] = bf16_pair(v[i + 2 * j], v[i + 2 * j + 1]);
+				store32(q + i, r);
 			}
 		}
 		if (h.db)
-			sums[wq][c + lane] = column_sums(v);
+			sums[threadIdx.x >> 5 & 3][c0 + c * 32 + lane] = column_sums(v);
+		asm volatile("" ::: "memory");	/* one 32 after the other: what is read ahead is spilled */
 	}
 	if (h.db) {
+		const int i = epi_thread();
+
 		epi_barrier();
-		for (int i = threadIdx.x & 127; i < HEAD_TN; i += 128)
-			if (at.m0 < h.tokens && h.v0 + at.n0 + i < h.v1)
-				h.dbp[(int64_t)(at.m0 / HEAD_HALF) * h.vocab + h.v0 + at.n0 + i] =
-				    (sums[0][i] + sums[1][i]) + (sums[2][i] + sums[3][i]);
+		if (at.m0 < h.tokens && h.v0 + at.n0 + i < h.v1)
+			h.dbp[(int64_t)(at.m0 / HEAD_HALF) * h.vocab + h.v0 + at.n0 + i] =
+			    (sums[0][i] + sums[1][i]) + (sums[2][i] + sums[3][i]);
 	}
 }
 
@@ -557,38 +605,40 @@ __device__ __forceinline__ void put_row(void *base, int64_t first, const float (
 	}
 }
 
-__device__ __forceinline__ void dx_epilogue(const gemm_args &g, const tile_at &at, uint32_t tmem, bool ok)
+__device__ __forceinline__ void dx_epilogue(const gemm_args &g, const tile_at &at, float (&acc)[4][32])
 {
 	const head_args &h = g.h;
-	const int t = at.m0 + (threadIdx.x & 127);
+	const int t = at.m0 + epi_row();
 
-#pragma unroll 1
-	for (int c = 0; c < HEAD_TN && at.n0 + c < h.d; c += 32) {
-		float v[32];
+	if (t >= h.tokens)
+		return;
+#pragma unroll
+	for (int c = 0; c < 4; c++) {
+		const int d = at.n0 + epi_col() + c * 32;
 
-		tmem_load(tmem + c, ok, v);
-		if (t >= h.tokens)
-			continue;
+		if (d >= h.d)
+			break;
 		if (h.dxp)
-			put_row(h.dxp, ((int64_t)at.split * h.tokens + t) * h.ldd + at.n0 + c, v, h.ldd - at.n0 - c, false, h.v0 != 0);
+			put_row(h.dxp, ((int64_t)at.split * h.tokens + t) * h.ldd + d, acc[c], h.ldd - d, false, h.v0 != 0);
 		else		/* one part, one piece: that is dx */
-			put_row(h.dx, t * h.lddx + at.n0 + c, v, h.d - at.n0 - c, h.bf16, false);
+			put_row(h.dx, t * h.lddx + d, acc[c], h.d - d, h.bf16, false);
 	}
 }
 
-__device__ __forceinline__ void dw_epilogue(const gemm_args &g, const tile_at &at, uint32_t tmem, bool ok)
+__device__ __forceinline__ void dw_epilogue(const gemm_args &g, const tile_at &at, float (&acc)[4][32])
 {
 	const head_args &h = g.h;
-	const int d = at.m0 + (threadIdx.x & 127);
-	const int v0 = h.v0 + at.n0;
+	const int d = at.m0 + epi_row();
 
-#pragma unroll 1
-	for (int c = 0; c < HEAD_TN && v0 + c < h.v1; c += 32) {
-		float v[32];
+	if (d >= h.d)
+		return;
+#pragma unroll
+	for (int c = 0; c < 4; c++) {
+		const int v = h.v0 + at.n0 + epi_col() + c * 32;
 
-		tmem_load(tmem + c, ok, v);
-		if (d < h.d)
-			put_row(h.dw, (int64_t)d * h.lddw + v0 + c, v, h.v1 - v0 - c, h.bf16, h.add);
+		if (v >= h.v1)
+			break;
+		put_row(h.dw, (int64_t)d * h.lddw + v, acc[c], h.v1 - v, h.bf16, h.add);
 	}
 }
 
@@ -612,32 +662,44 @@ struct gemm_smem {
 template <int KIND>
 __device__ __forceinline__ void producer(const gemm_args &g, gemm_smem *s, uint32_t ring, int total, int rank, int pair, int pairs)
 {
+	const int terms = KIND == DX || KIND == DW ? g.h.terms : 1;
 	uint32_t n = 0;		/* stages loaded so far */
 
 	for (int tile = pair; tile < total; tile += pairs) {
 		const tile_at at = tile_of<KIND>(g, tile, rank);
 
-		for (int term = 0; term < (KIND == DX || KIND == DW ? g.h.terms : 1); term++)
-			for (int k = at.k0; k < at.k1; k++, n++) {
-				const uint32_t i = n % HEAD_STAGES;
+		int k = at.k0;
+		int term = 0;
+		int from = k;	/* of this run */
 
-				if (!mbar_wait(smem_of(&s->empty[i]), (n / HEAD_STAGES & 1) ^ 1, &s->stop)) {
-					if (rank == 0)
-						for (uint32_t j = n < HEAD_STAGES ? 0 : n - HEAD_STAGES; j < n; j++)
-							(void)mbar_wait(smem_of(&s->full[j % HEAD_STAGES]),
-							    j / HEAD_STAGES & 1, NULL);
-					else {
-						/* counted elsewhere: no copy is under way for this long */
-						for (const uint64_t end = now_ns() + HEAD_WAIT_NS / 100; now_ns() < end; )
-							__nanosleep(1000);
-					}
-					return;
-				}
+		/* all terms of a run, the small ones first, then the next run */
+		while (from < at.k1) {
+			const uint32_t i = n % HEAD_STAGES;
+
+			if (!mbar_wait(smem_of(&s->empty[i]), (n / HEAD_STAGES & 1) ^ 1, &s->stop)) {
 				if (rank == 0)
-					mbar_expect(smem_of(&s->full[i]), 2 * HEAD_STAGE_BYTES);
-				load_stage<KIND>(g, at, KIND == DX || KIND == DW ? g.h.terms - 1 - term : 0, k * HEAD_TK,
-				    ring + i * HEAD_STAGE_BYTES, smem_in(smem_of(&s->full[i]), 0));
+					for (uint32_t j = n < HEAD_STAGES ? 0 : n - HEAD_STAGES; j < n; j++)
+						(void)mbar_wait(smem_of(&s->full[j % HEAD_STAGES]), j / HEAD_STAGES & 1, NULL);
+				else {
+					/* counted elsewhere: no copy is under way for this long */
+					for (const uint64_t end = now_ns() + HEAD_WAIT_NS / 100; now_ns() < end; )
+						__nanosleep(1000);
+				}
+				return;
 			}
+			if (rank == 0)
+				mbar_expect(smem_of(&s->full[i]), 2 * HEAD_STAGE_BYTES);
+			load_stage<KIND>(g, at, terms - 1 - term, k * HEAD_TK, ring + i * HEAD_STAGE_BYTES,
+			    smem_in(smem_of(&s->full[i]), 0));
+			n++;
+			if (++k == min(from + g.run, at.k1)) {
+				if (++term == terms) {
+					term = 0;
+					from = k;
+				}
+				k = from;
+			}
+		}
 	}
 }
 
@@ -649,36 +711,42 @@ __device__ __forceinline__ void multiplier(const gemm_args &g, gemm_smem *s, uin
 	const bool b_mn = KIND != DX;
 	const uint32_t idesc = instr_desc(a_mn, b_mn);
 	uint32_t n = 0;
-	uint32_t done = 0;	/* tiles */
+	uint32_t done = 0;	/* runs */
 
-	for (int tile = pair; tile < total; tile += pairs, done++) {
+	for (int tile = pair; tile < total; tile += pairs) {
 		const tile_at at = tile_of<KIND>(g, tile, 0);
-		const int steps = (at.k1 - at.k0) * (KIND == DX || KIND == DW ? g.h.terms : 1);
-		const uint32_t acc = s->tmem + (done & 1) * HEAD_TN;
-		bool ok = mbar_wait(smem_of(&s->drained[done & 1]), (done / 2 & 1) ^ 1, &s->stop);
 
-		asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-		for (int k = 0; ok && k < steps; k++, n++) {
-			const uint32_t i = n % HEAD_STAGES;
-			const uint32_t base = ring + i * HEAD_STAGE_BYTES;
+		for (int from = at.k0; from < at.k1; from += g.run, done++) {
+			const int steps = (min(from + g.run, at.k1) - from) * (KIND == DX || KIND == DW ? g.h.terms : 1);
+			const uint32_t acc = s->tmem + (done & 1) * HEAD_TN;
+			bool ok = mbar_wait(smem_of(&s->drained[done & 1]), (done / 2 & 1) ^ 1, &s->stop);
 
-			ok = mbar_wait(smem_of(&s->full[i]), n / HEAD_STAGES & 1, &s->stop);
-			if (!ok)
-				break;
 			asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-			/* 16 k a time: 32 bytes further in a K-major row, 16 rows of 128 bytes further in an MN-major box */
+			for (int k = 0; ok && k < steps; k++, n++) {
+				const uint32_t i = n % HEAD_STAGES;
+				const uint32_t base = ring + i * HEAD_STAGE_BYTES;
+
+				ok = mbar_wait(smem_of(&s->full[i]), n / HEAD_STAGES & 1, &s->stop);
+				if (!ok)
+					break;
+				asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+				/*
+				** 16 k a time: 32 bytes further in a K-major row, 16 rows of 128 bytes further in an
+				** MN-major box
+				*/
 #pragma unroll
-			for (int j = 0; j < HEAD_TK / 16; j++)
-				mma(acc, smem_desc(base + j * (a_mn ? 2048 : 32), a_mn),
-				    smem_desc(base + HEAD_A_BYTES + j * (b_mn ? 2048 : 32), b_mn), idesc, k > 0 || j > 0);
-			mma_commit(smem_of(&s->empty[i]));
+				for (int j = 0; j < HEAD_TK / 16; j++)
+					mma(acc, smem_desc(base + j * (a_mn ? 2048 : 32), a_mn),
+					    smem_desc(base + HEAD_A_BYTES + j * (b_mn ? 2048 : 32), b_mn), idesc, k > 0 || j > 0);
+				mma_commit(smem_of(&s->empty[i]));
+			}
+			if (!ok) {
+				mma_commit(smem_of(&s->quiet));
+				(void)mbar_wait(smem_of(&s->quiet), 0, NULL);
+				return;
+			}
+			mma_commit(smem_of(&s->ready[done & 1]));
 		}
-		if (!ok) {
-			mma_commit(smem_of(&s->quiet));
-			(void)mbar_wait(smem_of(&s->quiet), 0, NULL);
-			return;
-		}
-		mma_commit(smem_of(&s->ready[done & 1]));
 	}
 }
 
@@ -687,32 +755,60 @@ __device__ __forceinline__ void drainer(const gemm_args &g, gemm_smem *s, int to
 {
 	const uint32_t lanes = (uint32_t)(threadIdx.x >> 5 & 3) << 21;	/* this warp's quarter of the lanes: 32 w << 16 */
 	uint32_t done = 0;
+	uint32_t b = 0;
 
-	for (int tile = pair; tile < total; tile += pairs, done++) {
+	for (int tile = pair; tile < total; tile += pairs, b ^= 1) {
 		const tile_at at = tile_of<KIND>(g, tile, rank);
-		const uint32_t b = done & 1;
-		const uint32_t acc = s->tmem + lanes + b * HEAD_TN;
+		float acc[4][32];
 
 		if (KIND == LOSS)
 			stage_bias(g.h, at.n0, g.h.vocab, s->epi.bias[b]);
 		if (KIND == DELTA)
 			stage_bias(g.h, g.h.v0 + at.n0, g.h.v1, s->epi.bias[b]);
-		/* the whole warp waits; it keeps step with the other warps even after a give-up, for the barriers' sake */
-		const bool ok = __all_sync(0xffffffffu, mbar_wait(smem_of(&s->ready[b]), done / 2 & 1, &s->stop));
+#pragma unroll 1
+		for (int from = at.k0; from < at.k1; from += g.run, done++) {
+			const uint32_t addr = s->tmem + lanes + (done & 1) * HEAD_TN + epi_col();
 
-		asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-		if (KIND == LOSS)
-			loss_epilogue(g, at, acc, ok, s->epi.bias[b]);
-		else if (KIND == DELTA)
-			delta_epilogue(g, at, acc, ok, s->epi.bias[b], s->epi.sums[b]);
-		else if (KIND == DX)
-			dx_epilogue(g, at, acc, ok);
-		else
-			dw_epilogue(g, at, acc, ok);
-		asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+			/* the warps keep step with each other even after a give-up, for the barriers' sake */
+			(void)__all_sync(0xffffffffu, mbar_wait(smem_of(&s->ready[done & 1]), done / 2 & 1, &s->stop));
+			asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+			if (from == at.k0) {
+#pragma unroll
+				for (int c = 0; c < 4; c++)
+					tmem_load(addr + c * 32, acc[c]);
+#pragma unroll
+				for (int c = 0; c < 4; c++)
+					tmem_wait(acc[c]);
+			} else {
+#pragma unroll
+				for (int c = 0; c < 4; c++) {
+					float v[32];
+
+					tmem_load(addr + c * 32, v);
+					tmem_wait(v);
+#pragma unroll
+					for (int i = 0; i < 32; i++)
+						acc[c][i] += v[i];
+				}
+			}
+			asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+			__syncwarp();
+			if ((threadIdx.x & 31) == 0)
+				mbar_arrive_in(smem_in(smem_of(&s->drained[done & 1]), 0));
+		}
+		if (*static_cast<volatile int *>(&s->stop))	/* somebody gave up: nothing here is to be believed */
+#pragma unroll
+			for (int i = 0; i < 128; i++)
+				acc[i / 32][i % 32] = NAN;
 		__syncwarp();
-		if ((threadIdx.x & 31) == 0)
-			mbar_arrive_in(smem_in(smem_of(&s->drained[b]), 0));
+		if (KIND == LOSS)
+			loss_epilogue(g, at, acc, s->epi.bias[b], s->epi.half[b]);
+		else if (KIND == DELTA)
+			delta_epilogue(g, at, acc, s->epi.bias[b], s->epi.sums[b]);
+		else if (KIND == DX)
+			dx_epilogue(g, at, acc);
+		else
+			dw_epilogue(g, at, acc);
 	}
 }
 
@@ -746,7 +842,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HEAD_THREADS, 1) pro
 		}
 		for (int i = 0; i < 2; i++) {
 			mbar_init(smem_of(&s.ready[i]), 1);
-			mbar_init(smem_of(&s.drained[i]), 8);	/* four warps of either block */
+			mbar_init(smem_of(&s.drained[i]), 2 * HEAD_EPI / 32);	/* the warps of both blocks */
 		}
 		mbar_init(smem_of(&s.quiet), 1);
 		s.stop = 0;
@@ -763,13 +859,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HEAD_THREADS, 1) pro
 	cluster_barrier();
 	asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 	dependent();
-	if (warp == 0) {
-		if ((threadIdx.x & 31) == 0)
+	if (warp < 4) {
+		if (warp == 0 && (threadIdx.x & 31) == 0)
 			producer<KIND>(g, &s, ring, total, rank, pair, pairs);
-	} else if (warp == 1) {
-		if ((threadIdx.x & 31) == 0 && rank == 0)
+		if (warp == 1 && (threadIdx.x & 31) == 0 && rank == 0)
 			multiplier<KIND>(g, &s, ring, total, pair, pairs);
-	} else if (warp >= 4)
+	} else
 		drainer<KIND>(g, &s, total, rank, pair, pairs);
 	__syncwarp();
 	asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -1211,6 +1306,8 @@ int product(const head_args &h, cudaStream_t st)
 		rc = tensor_map(&g.a, h.x, h.d, h.tokens, h.ldx, 1, HEAD_TK);
 		rc = rc ? rc : tensor_map(&g.b, h.delta, width, h.tokens, h.ldp, h.terms, HEAD_TK);
 	}
+	/* the losses and fp32 gradients are to be good to fp32; what is rounded to bf16 has no use for it */
+	g.run = KIND == LOSS || (KIND == DELTA && h.terms > 1) ? HEAD_RUN : h.terms > 1 ? HEAD_RUN_F32 : g.k_blocks;
 	if (rc != ANNI_OK)
 		return rc;
 	rc = ready(product_kernel<KIND>, smem, &sms, &known[KIND]);
