@@ -51,6 +51,7 @@
 #define HEAD_PAIRS	74	/* pairs of SMs that the work is cut for; any number of them runs it */
 #define HEAD_PIECE_BYTES ((size_t)256 << 20)	/* of delta in the workspace */
 #define HEAD_TERMS	3	/* bf16 terms of delta for fp32 gradients */
+#define HEAD_FEW_DIM	8192	/* rows_kernel keeps two rows of x in shared memory */
 #define HEAD_WAIT_NS	2000000000ull	/* a wait inside a kernel gives up after this long */
 
 namespace {
@@ -875,9 +876,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HEAD_THREADS, 1) pro
 		asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" :: "r"(s.tmem) : "memory");
 }
 
-/* ---- what goes before and after the products ------------------------------------------------------------ */
-
-/* joins the tiles of a row: 32 warps share the tiles of 32 rows */
+/* maximum and sum of one part of a row taken into those of the others */
 __device__ __forceinline__ void join(float &top, float &sum, float2 p)
 {
 	const float high = fmaxf(top, p.x);
@@ -887,6 +886,126 @@ __device__ __forceinline__ void join(float &top, float &sum, float2 p)
 	top = high;
 }
 
+/* ---- a few rows ------------------------------------------------------------------------------------------- */
+
+/*
+** The loss of one row or two: W is read once and little is computed, so HBM is the bound, and a product whose
+** tiles have 256 rows spends longer on the empty ones (1536 x 100,000: one row 93 us there and 65 us here, two rows
+** 91 and 64, four rows 92 and 119; reading W alone takes 47 us).  A block takes 256 entries of the vocabulary, each
+** of its eight warps an eighth of the rows of W: ROWS x 8 sums a thread, in fp32, added up over the warps in
+** order.  VEC: lane l has columns 8 l .. 8 l + 7, else (no 16-byte grid) columns l, l + 32, ...
+*/
+template <int ROWS, bool VEC>
+__global__ void __launch_bounds__(256) rows_kernel(const head_args h)
+{
+	extern __shared__ float xs[];		/* [d][ROWS] */
+	__shared__ float red[8][HEAD_TN];
+	__shared__ float2 warps[8];
+	const int lane = threadIdx.x & 31;
+	const int w = threadIdx.x >> 5;
+	const int v0 = blockIdx.x * HEAD_TN;
+	const int lo = (int)((int64_t)h.d * w / 8);
+	const int hi = (int)((int64_t)h.d * (w + 1) / 8);
+	const int mine = v0 + threadIdx.x;
+	float acc[ROWS][8];
+
+	dependent();
+	for (int i = threadIdx.x; i < h.d * ROWS; i += 256)
+		xs[i] = to_f(h.x[(int64_t)(i % ROWS) * h.ldx + i / ROWS]);
+#pragma unroll
+	for (int r = 0; r < ROWS; r++)
+#pragma unroll
+		for (int j = 0; j < 8; j++)
+			acc[r][j] = 0.0f;
+	__syncthreads();
+	for (int d0 = lo; d0 < hi; d0 += 8) {
+		uint32_t q[8][4];
+
+#pragma unroll
+		for (int k = 0; k < 8; k++) {
+			const __nv_bfloat16 *row = h.w + (int64_t)(d0 + k) * h.ldw + v0;
+
+#pragma unroll
+			for (int j = 0; j < 4; j++)
+				q[k][j] = 0;
+			if (d0 + k >= hi)
+				continue;
+			if (VEC && v0 + lane * 8 + 8 <= h.vocab) {
+				const uint4 r = __ldcs(reinterpret_cast<const uint4 *>(row + lane * 8));
+
+				q[k][0] = r.x;
+				q[k][1] = r.y;
+				q[k][2] = r.z;
+				q[k][3] = r.w;
+			} else
+#pragma unroll
+				for (int j = 0; j < 8; j++) {
+					const int c = VEC ? lane * 8 + j : lane + 32 * j;
+
+					if (v0 + c < h.vocab)
+						q[k][j / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(row)[c] << (j % 2 * 16);
+				}
+		}
+#pragma unroll
+		for (int k = 0; k < 8; k++) {
+			if (d0 + k >= hi)
+				break;
+#pragma unroll
+			for (int j = 0; j < 8; j += 2) {
+				const float2 b = unpack2(q[k][j / 2]);
+
+#pragma unroll
+				for (int r = 0; r < ROWS; r++) {
+					const float a = xs[(d0 + k) * ROWS + r];
+
+					acc[r][j] = fmaf(a, b.x, acc[r][j]);
+					acc[r][j + 1] = fmaf(a, b.y, acc[r][j + 1]);
+				}
+			}
+		}
+	}
+#pragma unroll
+	for (int r = 0; r < ROWS; r++) {
+		float z = 0.0f;
+		float top;
+		float sum;
+
+		__syncthreads();
+#pragma unroll
+		for (int j = 0; j < 8; j++)
+			red[w][VEC ? lane * 8 + j : lane + 32 * j] = acc[r][j];
+		__syncthreads();
+#pragma unroll
+		for (int k = 0; k < 8; k++)
+			z += red[k][threadIdx.x];
+		if (mine >= h.vocab)
+			z = -INFINITY;
+		else if (h.bias)
+			z += h.bias[mine];
+		if (mine < h.vocab && h.target[r] == mine)
+			h.hit[r] = z;
+		top = z;
+#pragma unroll
+		for (int k = 16; k > 0; k >>= 1)
+			top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+		sum = exp2_approx((z - (top == -INFINITY ? 0.0f : top)) * LOG2E);
+#pragma unroll
+		for (int k = 16; k > 0; k >>= 1)
+			sum += __shfl_xor_sync(0xffffffffu, sum, k);
+		if (lane == 0)
+			warps[w] = make_float2(top, sum);
+		__syncthreads();
+		if (threadIdx.x == 0) {
+			for (int k = 1; k < 8; k++)
+				join(top, sum, warps[k]);
+			h.part[(int64_t)blockIdx.x * h.tokens + r] = make_float2(top, sum);
+		}
+	}
+}
+
+/* ---- what goes before and after the products ------------------------------------------------------------ */
+
+/* joins the tiles of a row: 32 warps share the tiles of 32 rows */
 __global__ void __launch_bounds__(1024) join_kernel(const head_args h, int tiles)
 {
 	__shared__ float2 s[32][33];
@@ -1020,10 +1139,17 @@ int64_t up(int64_t n, int64_t to)
 	return (n + to - 1) / to * to;
 }
 
+/* the loss by rows_kernel, which takes x and w as they are */
+bool few_rows(const anni_head_call *c)
+{
+	return c->tokens <= 2 && c->d_model <= HEAD_FEW_DIM;
+}
+
 /* where things lie in the workspace (byte offsets), and how the work is cut */
 struct head_plan {
 	size_t	x;		/* copies of x and w on a 16-byte grid, where needed */
 	size_t	w;
+	int	few;		/* rows_kernel */
 	int	copy_x;
 	int	copy_w;
 	int64_t	ldx;
@@ -1111,8 +1237,9 @@ head_plan plan_of(const anni_head_call *c, int grad)
 	const int64_t t = std::max<int64_t>(c->tokens, 1);
 
 	memset(&p, 0, sizeof(p));
-	p.copy_x = grad || (c->ldx & 7) || ((uintptr_t)c->x & 15);
-	p.copy_w = (c->ldw & 7) || ((uintptr_t)c->w & 15);
+	p.few = !grad && few_rows(c);
+	p.copy_x = grad || (!p.few && ((c->ldx & 7) || ((uintptr_t)c->x & 15)));
+	p.copy_w = !p.few && ((c->ldw & 7) || ((uintptr_t)c->w & 15));
 	p.ldx = up(c->d_model, 8);
 	p.ldw = up(c->vocab, 8);
 	p.x = take(&p.bytes, p.copy_x ? t * p.ldx * 2 : 0);
@@ -1253,6 +1380,7 @@ int tensor_map(CUtensorMap *m, const void *base, int64_t cols, int64_t rows, int
 */
 #define HEAD_DEVICES	16
 std::atomic<int> known[4][HEAD_DEVICES];
+std::atomic<int> known_rows[2][2][HEAD_DEVICES];
 
 template <typename K>
 int ready(K kernel, int smem, int *sms, std::atomic<int> (*seen)[HEAD_DEVICES])
@@ -1317,6 +1445,20 @@ int product(const head_args &h, cudaStream_t st)
 	    smem, st, g);
 }
 
+template <int ROWS>
+int loss_rows(const head_args &h, bool vec, cudaStream_t st)
+{
+	const int smem = h.d * ROWS * 4;
+	int sms;
+	int rc = vec ? ready(rows_kernel<ROWS, true>, ROWS * HEAD_FEW_DIM * 4, &sms, &known_rows[ROWS - 1][1])
+	    : ready(rows_kernel<ROWS, false>, ROWS * HEAD_FEW_DIM * 4, &sms, &known_rows[ROWS - 1][0]);
+
+	if (rc != ANNI_OK)
+		return rc;
+	return vec ? launch(rows_kernel<ROWS, true>, tiles(h.vocab, HEAD_TN), 256, smem, st, h)
+	    : launch(rows_kernel<ROWS, false>, tiles(h.vocab, HEAD_TN), 256, smem, st, h);
+}
+
 /* the copies that the plan asks for; x's with the factors of the rows when gradients follow */
 int pack(const anni_head_call *c, const head_plan &p, const head_args &h, bool grad, cudaStream_t st)
 {
@@ -1364,7 +1506,11 @@ extern "C" int anni_head_loss(const anni_head_call *c, void *stream)
 	h = args_of(c, p);
 	rc = pack(c, p, h, false, st);
 	h.v1 = h.vocab;
-	if (rc == ANNI_OK)
+	if (rc == ANNI_OK && p.few) {
+		const bool vec = (h.ldw & 7) == 0 && ((uintptr_t)h.w & 15) == 0;
+
+		rc = h.tokens == 1 ? loss_rows<1>(h, vec, st) : loss_rows<2>(h, vec, st);
+	} else if (rc == ANNI_OK)
 		rc = product<LOSS>(h, st);
 	if (rc == ANNI_OK)
 		rc = launch(join_kernel, tiles(h.tokens, 32), 1024, 0, st, h, (int)tiles(h.vocab, HEAD_TN));

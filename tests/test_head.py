@@ -105,7 +105,8 @@ def both(x, w, target, b, kind, weight=None, scale=1.0):
 
 
 SHAPES = [(1, 1, 1), (1, 64, 300), (2, 8, 8), (5, 3, 7), (127, 64, 300), (128, 64, 256), (129, 65, 257), (300, 200, 1000),
-          (257, 136, 5003), (64, 1536, 4096), (1000, 72, 264), (3, 520, 20001)]
+          (257, 136, 5003), (64, 1536, 4096), (1000, 72, 264), (3, 520, 20001), (8, 1536, 1000), (4, 64, 512), (7, 100, 777),
+          (8, 2056, 264), (9, 64, 300)]
 
 
 @gpu
@@ -223,6 +224,8 @@ def test_masked_vocabulary(kind):
     ex = Exact(x, w, target, b)
     check_loss(ex, nll, lse)
     check_grads(ex, kind, dx=dx, dw=dw, db=db)
+    few = Exact(x[:5], w, target[:5], b)
+    check_loss(few, *head_loss(x[:5], w, target[:5], bias=b))
     assert not dw[:, :700].any() and not db[1490:].any()
     target[0] = 3
     nll, lse, dx, dw, db = both(x, w, target, b, kind)
@@ -260,6 +263,8 @@ def test_nan_row_with_a_target():
     assert torch.isnan(nll[7])
     nll[7] = clean[7]
     assert torch.equal(nll, clean)
+    few, _ = head_loss(x[4:8], w, target[4:8], bias=b)
+    assert torch.isnan(few[3]) and torch.isfinite(few[:3]).all()
 
 
 @gpu
