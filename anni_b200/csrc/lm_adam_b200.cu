@@ -16,6 +16,7 @@
 #include <thread>
 #include <vector>
 #include "anni_gpu_compat.h"
+#include "anni_head.h"
 #include "anni_lm_adam.h"
 #include "optstep_internal.h"
 
@@ -434,6 +435,39 @@ extern "C" int anni_lm_adam_alias_vec(anni_lm_adam *opt, int tensor, float **d_w
 		*d_w = opt->d_param + s->off;
 	if (d_dw)
 		*d_dw = grad_slice;
+	return ANNI_OK;
+}
+
+extern "C" int anni_lm_adam_head_call(const anni_lm_adam *opt, int w_tensor, int b_tensor, anni_head_call *c)
+{
+	const anni_lm_adam_seg *w;
+	const anni_lm_adam_seg *b = NULL;
+	size_t size;
+
+	if (!opt || !c || w_tensor < 0 || w_tensor >= opt->n_segs || b_tensor >= opt->n_segs || b_tensor == w_tensor)
+		return ANNI_E_ARG;
+	if (!opt->d_param || !opt->d_param_bf16 || !opt->d_grad || !opt->params_valid
+	    || (opt->n > 0x7fffffff && opt->t == 0))
+		return ANNI_E_ARG;		/* the twin does not hold the weights (yet) */
+	w = &opt->segs[w_tensor];
+	if (c->d_model < 1 || c->vocab < 1 || w->n != (int64_t)c->d_model * c->vocab || w->dw
+	    || !(w->flags & ANNI_SEG_TWIN_BF16))
+		return ANNI_E_ARG;
+	if (b_tensor >= 0) {
+		b = &opt->segs[b_tensor];
+		if (b->n != c->vocab || b->dw)
+			return ANNI_E_ARG;
+	}
+	size = elem_size(opt->grad_dtype);
+	c->w = (const uint16_t *)opt->d_param_bf16 + w->off;
+	c->ldw = c->vocab;
+	c->bias = b ? opt->d_param + b->off : NULL;
+	c->grad_scale = opt->loss_scale > 0.0 ? opt->loss_scale : 1.0;
+	c->grad_dtype = opt->grad_dtype;
+	c->flags = ANNI_HEAD_ACCUMULATE;
+	c->dw = (char *)opt->d_grad + (size_t)w->off * size;
+	c->lddw = c->vocab;
+	c->dbias = b ? (char *)opt->d_grad + (size_t)b->off * size : NULL;
 	return ANNI_OK;
 }
 

@@ -339,6 +339,34 @@ class OptStep:
         if self.has_fp8:
             self.quantize(stream)
 
+    def head_loss(self, x, target, *, w="w_head", b="b_head", weight=None, grad_scale=1.0, grad=True, dx=None,
+                  stream=None):
+        """Loss of the head whose weights this engine steps: rows of nll for x (tokens, d_model) bf16 against
+        ``target`` (tokens) int32, W read from the tensor ``w``'s twin, the bias (``b`` or None) from the master;
+        with ``grad`` the gradients of ``grad_scale * sum(weight * nll)`` are added to the engine's gradients and,
+        if ``dx`` is given, written there (see anni_b200.head)."""
+        from .head import head_loss, head_loss_grad
+        if self.segments is None or self.shard_off != 0 or self.shard_n != self.n_arena:
+            raise ValueError("head_loss: needs an engine over a whole arena with named tensors")
+        if self.twin_bf16 is None or not self.segments.flags[self.segments.index(w)] & SEG_TWIN_BF16:
+            raise ValueError(f"head_loss: tensor {w} has no bf16 twin")
+        at = self.segments.slice_of(w)
+        d = x.shape[1]
+        if (at.stop - at.start) % d:
+            raise ValueError(f"head_loss: tensor {w} has no rows of {d}")
+        at_b = self.segments.slice_of(b) if b is not None else None
+        wt = self.twin_bf16[at].view(d, -1)
+        bias = self.master[at_b] if b is not None else None
+        nll, lse = head_loss(x, wt, target, bias=bias, stream=stream)
+        if grad or dx is not None:
+            g = self.grad
+            kw = dict(dw=g[at].view(d, -1), dbias=g[at_b] if b is not None else None) if grad else {}
+            if dx is not None and dx.dtype != g.dtype:
+                raise TypeError("head_loss: dx has the type of the engine's gradients")
+            head_loss_grad(x, wt, target, lse, bias=bias, weight=weight, grad_scale=grad_scale, dx=dx, accumulate=True,
+                           stream=stream, **kw)
+        return nll
+
     # -- small device buffers as tensors (for collectives) -----------------------------------
     def _as_tensor(self, ptr, n, dtype):
         """A torch view of library-owned device memory (no copy, not owned by torch)."""

@@ -36,6 +36,8 @@ def lib():
         P = C.POINTER(Call)
         L.anni_head_workspace.restype = C.c_int
         L.anni_head_workspace.argtypes = [P, C.c_int, C.POINTER(C.c_size_t)]
+        L.anni_lm_adam_head_call.restype = C.c_int
+        L.anni_lm_adam_head_call.argtypes = [C.c_void_p, C.c_int, C.c_int, P]
         for f in (L.anni_head_loss, L.anni_head_loss_grad):
             f.restype = C.c_int
             f.argtypes = [P, C.c_void_p]

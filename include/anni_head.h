@@ -90,6 +90,18 @@ int	anni_head_loss(const anni_head_call *c, void *stream);
 /* dx, dw, dbias from lse, which an anni_head_loss on the same x, w, bias has written. */
 int	anni_head_loss_grad(const anni_head_call *c, void *stream);
 
+/*
+** The call's share of an optimizer object (anni_lm_adam.h): W is tensor w_tensor's bf16 twin, the bias tensor
+** b_tensor's fp32 weights (b_tensor < 0: none); dw and dbias are their slices of the gradient flat, added to as
+** the backward pass of the reference does (lang/lm_train.c:1220-1226), grad_scale is the object's loss
+** scale, grad_dtype its gradients' type.  The caller has set d_model and vocab and sets everything else
+** (x, target, tokens, nll, lse, weight, dx, workspace) before or after.  The flats live as long as the object;
+** its step reads and clears the gradients on the legacy stream: run the head there, or order the two.
+** ANNI_E_ARG: not prepared (anni_lm_adam_prepare) or invalidated, a tensor of another size, without a twin, or
+** whose gradients still come from the host (anni_lm_adam_alias / _alias_vec end that).
+*/
+int	anni_lm_adam_head_call(const anni_lm_adam *opt, int w_tensor, int b_tensor, anni_head_call *c);
+
 #ifdef __cplusplus
 }
 #endif

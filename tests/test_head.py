@@ -443,4 +443,4 @@ def test_workspace_is_bounded():
 def test_every_declared_symbol_is_exported():
     from test_abi_cpu import _declared_symbols
     names = _declared_symbols("anni_head.h")
-    assert len(names) == 3 and not [k for k in names if not hasattr(head.lib(), k)]
+    assert len(names) == 4 and not [k for k in names if not hasattr(head.lib(), k)]
