@@ -1,10 +1,10 @@
 /*
 ** AdamW over a list of tensors (include/anni_mtstep.h): one cooperative launch per step.
 **
-** The list is cut into tiles of ANNI_MT_TILE elements that do not cross tensors; a table says which
-** tensor a tile belongs to.  A block takes a tile at a time, each of its eight warps runs of
-** ANNI_MT_BLOCK = 256 elements -- the run that shares a scale in the 8-bit form, so that the two
-** block maxima are reductions inside a warp.  The step is bound by HBM: 28 bytes per element with 32-bit
+** Every tensor is cut into whole tiles of ANNI_MT_TILE elements, which a table lists with their tensors, and
+** what is left of it, which a second table lists: two loops, the first without a thought for ends.  A block
+** takes a tile at a time, each of its eight warps a run of ANNI_MT_BLOCK = 256 elements -- the run that
+** shares a scale in the 8-bit form, so that the two block maxima are reductions inside a warp.  The step is bound by HBM: 28 bytes per element with 32-bit
 ** moments, bf16 gradients and twins, 16 with 8-bit moments.
 */
 #include <cuda_bf16.h>
@@ -35,9 +35,8 @@ struct mt_desc {
 	uint16_t	*twin;		/* NULL: none */
 	int64_t		n;
 	uint64_t	block0;		/* blocks of 256 in the tensors before this one */
-	uint32_t	tile0;		/* tiles in the tensors before this one */
-	uint16_t	wd;
-	uint16_t	vec;		/* everything but the gradient on the alignment of the vector accesses */
+	uint32_t	tile0;		/* whole tiles in the tensors before this one */
+	uint32_t	wd;
 };
 
 static_assert(sizeof(mt_desc) % 8 == 0, "mt_held keeps the gradient's address behind it");
@@ -46,8 +45,10 @@ struct mt_launch {
 	anni_launch	la;		/* hyper-parameters, flags, control block */
 	const mt_desc	*desc;
 	void *const	*grad;
-	const uint32_t	*tile_of;	/* tensor of each tile */
+	const uint32_t	*tile_of;	/* tensor of each whole tile */
+	const uint32_t	*rest_of;	/* tensors that do not end with a whole tile */
 	uint32_t	tiles;
+	uint32_t	rests;
 	uint64_t	seed;
 	float		b1;		/* beta1, 1 - beta1, beta2, 1 - beta2 for the 8-bit form */
 	float		omb1;
@@ -110,12 +111,20 @@ __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b)
 	return r;
 }
 
+/*
+** Sums of products that are to be rounded on their own: two plain additions.  (The assembler contracts a packed
+** product and a packed sum into one fused operation, whatever rounding they name: checked on a million pairs.)
+*/
 __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b)
 {
-	f32x2 r;
+	float a0;
+	float a1;
+	float b0;
+	float b1;
 
-	asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-	return r;
+	unpair(a, a0, a1);
+	unpair(b, b0, b1);
+	return pair(__fadd_rn(a0, b0), __fadd_rn(a1, b1));
 }
 
 __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c)
@@ -158,7 +167,7 @@ __device__ __forceinline__ void q8_scale(uint32_t amax_bits, float top, float &s
 	const float amax = __uint_as_float(amax_bits);
 	const bool none = amax < 7.8886090522101181e-31f;	/* 2^-100 */
 
-	scale = none ? 0.0f : __fdiv_rn(amax, top);
+	scale = none ? 0.0f : __fmul_rn(amax, 1.0f / top);
 	inv = none ? 0.0f : __fmul_rn(__frcp_rn(amax), top);
 }
 
@@ -202,62 +211,58 @@ __device__ __forceinline__ void q8_round(bool random, uint32_t key, uint32_t i, 
 
 /*
 ** Tensors on addresses that only their type allows: element-wise, lane l on elements l, l + 32, ... of the
-** run, so that plain accesses coalesce.  One element at a time, which keeps its registers out of the way of the
-** vector path's.
+** run, so that plain accesses coalesce.
 */
 template <typename GradT, bool Q8>
 __device__ __forceinline__ void run_scalar(const mt_launch &a, const mt_desc &d, void *grad, int64_t e0, int len,
-	double coef, bool skip)
+	double coef)
 {
 	const int lane = threadIdx.x & 31;
 	const float lrwd = d.wd ? a.la.lrwd : 0.0f;
 	const int64_t blk = e0 / ANNI_MT_BLOCK;
+	const float old_ms = Q8 ? d.ms[blk] : 0.0f;
+	const float old_vs = Q8 ? d.vs[blk] : 0.0f;
 	float m[8];
 	float v[8];
-	float ms = 0.0f;
-	float vs = 0.0f;
 	uint32_t am = 0;
 	uint32_t av = 0;
 
-	if (!skip) {
-		if (Q8) {
-			ms = d.ms[blk];
-			vs = d.vs[blk];
-		}
 #pragma unroll
-		for (int j = 0; j < 8; j++) {
-			const int i = j * 32 + lane;
-			const int64_t e = e0 + i;
+	for (int j = 0; j < 8; j++) {
+		const int64_t e = e0 + j * 32 + lane;
 
-			m[j] = v[j] = 0.0f;
-			if (i < len) {
-				float p = d.p[e];
-				const float g = io8<GradT>::load1(grad, e);
+		m[j] = v[j] = 0.0f;
+		if (j * 32 + lane < len) {
+			float p = d.p[e];
+			const float g = io8<GradT>::load1(grad, e);
 
-				if (Q8) {
-					f32x2 m2 = pair(__fmul_rn(e4m3_to_float(static_cast<const uint8_t *>(d.m)[e]), ms), 0.0f);
-					f32x2 v2 = pair(__fmul_rn(e5m2_to_float(static_cast<const uint8_t *>(d.v)[e]), vs), 0.0f);
-					float none = 0.0f;
+			if (Q8) {
+				f32x2 m2 = pair(__fmul_rn(e4m3_to_float(static_cast<const uint8_t *>(d.m)[e]), old_ms), 0.0f);
+				f32x2 v2 = pair(__fmul_rn(e5m2_to_float(static_cast<const uint8_t *>(d.v)[e]), old_vs), 0.0f);
+				float none = 0.0f;
 
-					adam_q8(a, (float)coef, lrwd, g, 0.0f, p, none, m2, v2);
-					unpair(m2, m[j], none);
-					unpair(v2, v[j], none);
-					am = max(am, __float_as_uint(fabsf(m[j])));
-					av = max(av, __float_as_uint(v[j]));
-				} else {
-					m[j] = static_cast<const float *>(d.m)[e];
-					v[j] = static_cast<const float *>(d.v)[e];
-					adam_elem<false>(a.la, coef, lrwd, g, p, m[j], v[j]);
-					static_cast<float *>(d.m)[e] = m[j];
-					static_cast<float *>(d.v)[e] = v[j];
-				}
-				d.p[e] = p;
-				if (d.twin)
-					io8<__nv_bfloat16>::store1(d.twin, e, p);
+				adam_q8(a, (float)coef, lrwd, g, 0.0f, p, none, m2, v2);
+				unpair(m2, m[j], none);
+				unpair(v2, v[j], none);
+				am = max(am, __float_as_uint(fabsf(m[j])));
+				av = max(av, __float_as_uint(v[j]));
+			} else {
+				m[j] = static_cast<const float *>(d.m)[e];
+				v[j] = static_cast<const float *>(d.v)[e];
+				adam_elem<false>(a.la, coef, lrwd, g, p, m[j], v[j]);
+				static_cast<float *>(d.m)[e] = m[j];
+				static_cast<float *>(d.v)[e] = v[j];
 			}
+			d.p[e] = p;
+			if (d.twin)
+				io8<__nv_bfloat16>::store1(d.twin, e, p);
+			if (a.la.flags & ANNI_STEP_ZERO_GRAD)
+				io8<GradT>::store1(grad, e, 0.0f);
 		}
 	}
-	if (Q8 && !skip) {
+	if (Q8) {
+		float ms;
+		float vs;
 		float mi;
 		float vi;
 		uint32_t key = 0;
@@ -275,20 +280,16 @@ __device__ __forceinline__ void run_scalar(const mt_launch &a, const mt_desc &d,
 #pragma unroll
 		for (int j = 0; j < 8; j++) {
 			const int i = j * 32 + lane;
-
-			if (i >= len)
-				continue;
 			float x = __fmul_rn(m[j], mi);
 			float y = __fmul_rn(v[j], vi);
 
+			if (i >= len)
+				continue;
 			q8_round(a.la.flags & ANNI_STEP_STOCHASTIC, key, (uint32_t)i, v[j], vi, x, y);
 			static_cast<uint8_t *>(d.m)[e0 + i] = (uint8_t)to_e4m3(x);
 			static_cast<uint8_t *>(d.v)[e0 + i] = (uint8_t)to_e5m2(y);
 		}
 	}
-	if (a.la.flags & ANNI_STEP_ZERO_GRAD)
-		for (int i = lane; i < len; i += 32)
-			io8<GradT>::store1(grad, e0 + i, 0.0f);
 }
 
 /*
@@ -319,6 +320,33 @@ __device__ __forceinline__ void store_some(void *base, uint64_t e, const f32x4 &
 	for (int j = 0; j < 4; j++)
 		if (j < left)
 			io8<T>::store1(base, e + j, r.x[j]);
+}
+
+/* gradients: `vec` says whether their address allows the vector accesses */
+template <typename T, bool ALL>
+__device__ __forceinline__ f32x4 load_grad(const void *base, uint64_t e, int left, bool vec)
+{
+	f32x4 r;
+
+	if (vec)
+		return load_some<T, ALL>(base, e, left);
+#pragma unroll
+	for (int j = 0; j < 4; j++)
+		r.x[j] = ALL || j < left ? io8<T>::load1(base, e + j) : 0.0f;
+	return r;
+}
+
+template <typename T, bool ALL>
+__device__ __forceinline__ void zero_grad(void *base, uint64_t e, int left, bool vec)
+{
+	if (vec) {
+		store_some<T, ALL>(base, e, f32x4{}, left);
+		return;
+	}
+#pragma unroll
+	for (int j = 0; j < 4; j++)
+		if (ALL || j < left)
+			io8<T>::store1(base, e + j, 0.0f);
 }
 
 template <bool ALL>
@@ -364,6 +392,7 @@ __device__ __forceinline__ void run_vec_f32(const mt_launch &a, const mt_desc &d
 	void *const mp = d.m;
 	void *const vp = d.v;
 	uint16_t *const tp = d.twin;
+	const bool gvec = ((uintptr_t)grad & 15) == 0;
 
 #pragma unroll 1
 	for (int k = 0; k < 2; k++) {
@@ -373,7 +402,7 @@ __device__ __forceinline__ void run_vec_f32(const mt_launch &a, const mt_desc &d
 
 		if (!ALL && left <= 0)
 			break;
-		const f32x4 g = load_some<GradT, ALL>(grad, e, left);
+		const f32x4 g = load_grad<GradT, ALL>(grad, e, left, gvec);
 		f32x4 p = load_some<float, ALL>(pp, e, left);
 		f32x4 m = load_some<float, ALL>(mp, e, left);
 		f32x4 v = load_some<float, ALL>(vp, e, left);
@@ -387,7 +416,7 @@ __device__ __forceinline__ void run_vec_f32(const mt_launch &a, const mt_desc &d
 		if (tp)
 			store_some<__nv_bfloat16, ALL>(tp, e, p, left);
 		if (a.la.flags & ANNI_STEP_ZERO_GRAD)
-			store_some<GradT, ALL>(grad, e, f32x4{}, left);
+			zero_grad<GradT, ALL>(grad, e, left, gvec);
 	}
 }
 
@@ -419,6 +448,7 @@ __device__ __forceinline__ void run_vec_q8(const mt_launch &a, const mt_desc &d,
 	const float lrwd = d.wd ? a.la.lrwd : 0.0f;
 	const int64_t blk = e0 / ANNI_MT_BLOCK;
 	const uint64_t e = (uint64_t)e0 + lane * 4;
+	const bool gvec = ((uintptr_t)grad & 15) == 0;
 	const int left = len - lane * 4;	/* of this lane's four, and 128 more than of its second four */
 	f32x4 g[2];
 	f32x4 p[2];
@@ -435,7 +465,7 @@ __device__ __forceinline__ void run_vec_q8(const mt_launch &a, const mt_desc &d,
 
 #pragma unroll
 	for (int k = 0; k < 2; k++) {
-		g[k] = load_some<GradT, WHOLE>(grad, e + 128 * k, left - 128 * k);
+		g[k] = load_grad<GradT, WHOLE>(grad, e + 128 * k, left - 128 * k, gvec);
 		p[k] = load_some<float, WHOLE>(d.p, e + 128 * k, left - 128 * k);
 		qm[k] = load_codes<WHOLE>(d.m, e + 128 * k, left - 128 * k);
 		qv[k] = load_codes<WHOLE>(d.v, e + 128 * k, left - 128 * k);
@@ -463,7 +493,7 @@ __device__ __forceinline__ void run_vec_q8(const mt_launch &a, const mt_desc &d,
 		if (d.twin)
 			store_some<__nv_bfloat16, WHOLE>(d.twin, e + 128 * k, p[k], left - 128 * k);
 		if (a.la.flags & ANNI_STEP_ZERO_GRAD)
-			store_some<GradT, WHOLE>(grad, e + 128 * k, f32x4{}, left - 128 * k);
+			zero_grad<GradT, WHOLE>(grad, e + 128 * k, left - 128 * k, gvec);
 	}
 	am = __reduce_max_sync(0xffffffffu, am);
 	av = __reduce_max_sync(0xffffffffu, av);
@@ -516,33 +546,6 @@ __device__ __forceinline__ void run_vec_q8(const mt_launch &a, const mt_desc &d,
 	}
 }
 
-/* one tile: whole tiles, and runs of any length, on aligned addresses the fast way, other addresses element-wise */
-template <typename GradT, bool Q8>
-__device__ __forceinline__ void mt_tile(const mt_launch &a, const decision &dec, const mt_desc &d, void *grad,
-	uint32_t t, float (*slots)[2][ANNI_THREADS / 32], int &odd)
-{
-	const bool vec = d.vec && ((uintptr_t)grad & 15) == 0 && !dec.skip;
-	const int64_t first = (int64_t)(t - d.tile0) * ANNI_MT_TILE;
-	const int64_t e0 = first + (threadIdx.x >> 5) * ANNI_MT_BLOCK;
-	const int64_t left = d.n - e0;
-	const int len = left < ANNI_MT_BLOCK ? (int)left : ANNI_MT_BLOCK;
-
-	if (vec && first + ANNI_MT_TILE <= d.n) {
-		if (Q8) {
-			run_vec_q8<GradT, true>(a, d, grad, e0, len, (float)dec.coef, slots[odd]);
-			odd ^= 1;
-		} else
-			run_vec_f32<GradT, true>(a, d, grad, e0, len, dec.coef);
-	} else if (left <= 0)
-		return;
-	else if (!vec)
-		run_scalar<GradT, Q8>(a, d, grad, e0, len, dec.coef, dec.skip);
-	else if (Q8)
-		run_vec_q8<GradT, false>(a, d, grad, e0, len, (float)dec.coef, NULL);
-	else
-		run_vec_f32<GradT, false>(a, d, grad, e0, len, dec.coef);
-}
-
 /* the entry of a tensor in shared memory */
 struct mt_held {
 	mt_desc	d;
@@ -570,28 +573,27 @@ __device__ __forceinline__ void fetched(void)
 }
 
 /*
-** Blocks take tiles round-robin, backwards: the whole grid works inside one small window of every buffer, and
-** the gradients read last by the norm phase are the likeliest to sit in L2.  A tile's tensor is looked up one
-** tile ahead, its entry is loaded into shared memory while the tile before is worked on.
+** Blocks take the entries of a table round-robin, backwards: the whole grid works inside one small window of
+** every buffer, and the gradients read last by the norm phase are the likeliest to sit in L2.  An entry's tensor is
+** looked up one step ahead, what there is to know of it is loaded into shared memory while the entry before is
+** worked on.  work(tensor, gradient, entry) is called with the block together.
 */
-template <typename GradT, bool Q8>
-__device__ __forceinline__ void mt_update_phase(const mt_launch &a, const decision &dec)
+template <typename F>
+__device__ __forceinline__ void walk(const mt_launch &a, const uint32_t *table, uint32_t entries, mt_held (&held)[2], F work)
 {
-	__shared__ float slots[2][2][ANNI_THREADS / 32];	/* new scales of m and v, two tiles */
-	__shared__ mt_held held[2];				/* this tile's tensor and the next one */
 	const uint32_t G = gridDim.x;
-	uint32_t r = (a.tiles + G - 1) / G;
-	uint32_t s;		/* tensor of this tile */
+	uint32_t r = (entries + G - 1) / G;
+	uint32_t s;		/* tensor of this entry */
 	uint32_t next;		/* and of the next */
 	int cur = 0;
-	int odd = 0;
 
-	if (blockIdx.x >= a.tiles)
+	if (blockIdx.x >= entries)
 		return;
-	if ((r - 1) * G + blockIdx.x >= a.tiles)
+	if ((r - 1) * G + blockIdx.x >= entries)
 		r--;
-	s = a.tile_of[(r - 1) * G + blockIdx.x];
-	next = r > 1 ? a.tile_of[(r - 2) * G + blockIdx.x] : s;
+	s = table[(r - 1) * G + blockIdx.x];
+	next = r > 1 ? table[(r - 2) * G + blockIdx.x] : s;
+	__syncthreads();
 	fetch(a, s, held[0]);
 	fetched();
 	for (; r > 0; r--) {
@@ -600,15 +602,69 @@ __device__ __forceinline__ void mt_update_phase(const mt_launch &a, const decisi
 
 		s = next;
 		if (r > 2)
-			next = a.tile_of[t - 2 * G];
+			next = table[t - 2 * G];
 		if (change)
-			fetch(a, s, held[cur ^ 1]);	/* on its way while this tile is worked on */
+			fetch(a, s, held[cur ^ 1]);
 		if (held[cur].grad)
-			mt_tile<GradT, Q8>(a, dec, held[cur].d, held[cur].grad, t, slots, odd);
+			work(held[cur].d, held[cur].grad, t);
 		if (change) {
 			cur ^= 1;
 			fetched();
 		}
+	}
+}
+
+/*
+** ALIGNED: every address but the gradients' allows the vector accesses; otherwise everything goes element by
+** element.  A gradient's address may change between two replays of a captured step, so it is looked at here.
+*/
+template <typename GradT, bool Q8, bool ALIGNED>
+__device__ __forceinline__ void mt_update_phase(const mt_launch &a, const decision &dec)
+{
+	__shared__ float slots[2][2][ANNI_THREADS / 32];	/* new scales of m and v, two tiles */
+	__shared__ mt_held held[2];				/* this entry's tensor and the next one */
+	const int64_t mine = (threadIdx.x >> 5) * ANNI_MT_BLOCK;
+	const float coef = (float)dec.coef;
+	int odd = 0;
+
+	walk(a, a.tile_of, a.tiles, held, [&](const mt_desc &d, void *grad, uint32_t t) {
+		const int64_t e0 = (int64_t)(t - d.tile0) * ANNI_MT_TILE + mine;
+
+		if (!ALIGNED)
+			run_scalar<GradT, Q8>(a, d, grad, e0, ANNI_MT_BLOCK, dec.coef);
+		else if (Q8) {
+			run_vec_q8<GradT, true>(a, d, grad, e0, ANNI_MT_BLOCK, coef, slots[odd]);
+			odd ^= 1;
+		} else
+			run_vec_f32<GradT, true>(a, d, grad, e0, ANNI_MT_BLOCK, dec.coef);
+	});
+	walk(a, a.rest_of, a.rests, held, [&](const mt_desc &d, void *grad, uint32_t) {
+		const int64_t e0 = d.n / ANNI_MT_TILE * ANNI_MT_TILE + mine;
+		const int len = (int)min((int64_t)ANNI_MT_BLOCK, d.n - e0);
+
+		if (len <= 0)
+			return;
+		if (!ALIGNED)
+			run_scalar<GradT, Q8>(a, d, grad, e0, len, dec.coef);
+		else if (Q8)
+			run_vec_q8<GradT, false>(a, d, grad, e0, len, coef, NULL);
+		else
+			run_vec_f32<GradT, false>(a, d, grad, e0, len, dec.coef);
+	});
+}
+
+/* a skipped step that leaves the gradients zeroed */
+template <typename GradT>
+__device__ __forceinline__ void mt_zero_phase(const mt_launch &a)
+{
+	for (uint32_t t = blockIdx.x; t < a.tiles + a.rests; t += gridDim.x) {
+		const uint32_t s = t < a.tiles ? a.tile_of[t] : a.rest_of[t - a.tiles];
+		const int64_t n = a.desc[s].n;
+		const int64_t e0 = t < a.tiles ? (int64_t)(t - a.desc[s].tile0) * ANNI_MT_TILE : n / ANNI_MT_TILE * ANNI_MT_TILE;
+
+		if (a.grad[s])
+			for (int64_t e = e0 + threadIdx.x; e < min(n, e0 + ANNI_MT_TILE); e += ANNI_THREADS)
+				io8<GradT>::store1(a.grad[s], e, 0.0f);
 	}
 }
 
@@ -624,17 +680,19 @@ __device__ __forceinline__ double mt_norm_phase(const mt_launch &a)
 	double acc0 = 0.0;
 	double acc1 = 0.0;
 
-	for (uint32_t t = (threadIdx.x >> 5) * gridDim.x + blockIdx.x; t < a.tiles; t += step) {
-		const uint32_t s = a.tile_of[t];
+	for (uint32_t t = (threadIdx.x >> 5) * gridDim.x + blockIdx.x; t < a.tiles + a.rests; t += step) {
+		const bool whole = t < a.tiles;
+		const uint32_t s = whole ? a.tile_of[t] : a.rest_of[t - a.tiles];
 		const void *grad = a.grad[s];
-		const int64_t lo = (int64_t)(t - a.desc[s].tile0) * ANNI_MT_TILE;
-		const int64_t left = a.desc[s].n - lo;
-		const int len = left < ANNI_MT_TILE ? (int)left : ANNI_MT_TILE;
+		const int64_t n = a.desc[s].n;
+		const int64_t lo = whole ? (int64_t)(t - a.desc[s].tile0) * ANNI_MT_TILE : n / ANNI_MT_TILE * ANNI_MT_TILE;
+		const int len = whole ? ANNI_MT_TILE : (int)(n - lo);
+		const bool vec = ((uintptr_t)grad & 15) == 0;
 		int i = 0;
 
 		if (!grad)
 			continue;
-		if (((uintptr_t)grad & 15) == 0)
+		if (vec)
 			for (; i + 256 <= len; i += 1024) {
 				f32x8 g[4];
 
@@ -647,8 +705,8 @@ __device__ __forceinline__ double mt_norm_phase(const mt_launch &a)
 					if (i + 256 * k + 256 <= len)
 						norm_accumulate<GradT>(g[k], acc0, acc1);
 			}
-		/* what is left of the last 256, or everything on other alignments */
-		for (i = min(i, len & ~255); i < len; i += 256) {
+		/* what is left of the last 256, or everything on other addresses */
+		for (i = vec ? len & ~255 : 0; i < len; i += 256) {
 			float g[8];
 
 #pragma unroll
@@ -662,8 +720,12 @@ __device__ __forceinline__ double mt_norm_phase(const mt_launch &a)
 	return acc0 + acc1;
 }
 
-template <typename GradT, bool Q8>
-__global__ void __launch_bounds__(ANNI_THREADS, 4) mt_step_kernel(const mt_launch a)
+/*
+** Resident blocks per SM: as in the arena step, fewer where a thread has more bytes in flight (184.7 M elements,
+** 32-bit moments: 3 blocks 0.935 ms, 4 blocks 0.987 ms; 8-bit moments: 4 blocks 0.581 ms, 3 blocks 0.602 ms).
+*/
+template <typename GradT, bool Q8, bool ALIGNED>
+__global__ void __launch_bounds__(ANNI_THREADS, Q8 ? 4 : 3) mt_step_kernel(const mt_launch a)
 {
 	decision d;
 	double ss = 0.0;
@@ -685,8 +747,10 @@ __global__ void __launch_bounds__(ANNI_THREADS, 4) mt_step_kernel(const mt_launc
 		a.la.ctl->eff_scale = d.coef;
 		a.la.ctl->skipped = d.skip ? 1 : 0;
 	}
-	if (!d.skip || (a.la.flags & ANNI_STEP_ZERO_GRAD))
-		mt_update_phase<GradT, Q8>(a, d);
+	if (!d.skip)
+		mt_update_phase<GradT, Q8, ALIGNED>(a, d);
+	else if (a.la.flags & ANNI_STEP_ZERO_GRAD)
+		mt_zero_phase<GradT>(a);
 	step_epilogue(a.la.ctl, d.skip);
 }
 
@@ -701,13 +765,18 @@ __global__ void set_grads_kernel(void **to, const mt_addrs from, int n)
 		to[i] = from.g[i];
 }
 
-const void *step_kernel(int grad_dtype, int state_dtype)
+template <typename GradT, bool Q8>
+const void *step_kernel_of(bool aligned)
+{
+	return aligned ? (const void *)mt_step_kernel<GradT, Q8, true> : (const void *)mt_step_kernel<GradT, Q8, false>;
+}
+
+const void *step_kernel(int grad_dtype, int state_dtype, bool aligned)
 {
 	if (grad_dtype == ANNI_DT_BF16)
-		return state_dtype == ANNI_DT_Q8 ? (const void *)mt_step_kernel<__nv_bfloat16, true>
-		    : (const void *)mt_step_kernel<__nv_bfloat16, false>;
-	return state_dtype == ANNI_DT_Q8 ? (const void *)mt_step_kernel<float, true>
-	    : (const void *)mt_step_kernel<float, false>;
+		return state_dtype == ANNI_DT_Q8 ? step_kernel_of<__nv_bfloat16, true>(aligned)
+		    : step_kernel_of<__nv_bfloat16, false>(aligned);
+	return state_dtype == ANNI_DT_Q8 ? step_kernel_of<float, true>(aligned) : step_kernel_of<float, false>(aligned);
 }
 
 struct range {
@@ -768,6 +837,8 @@ struct anni_mtstep {
 	int			n_tensors;
 	int			blocks;
 	uint32_t		tiles;
+	uint32_t		rests;
+	bool			aligned;	/* everything but the gradients, which come and go */
 	anni_control		*ctl;		/* device, as the next three */
 	mt_desc			*desc;
 	void			**grad;
@@ -842,7 +913,8 @@ static int check_tensor(const anni_mt_tensor *t, int state_dtype, std::vector<ra
 static int create(const anni_mt_tensor *list, int n, anni_mtstep *h)
 {
 	std::vector<mt_desc> desc((size_t)n);
-	std::vector<uint32_t> tile_of;
+	std::vector<uint32_t> table;	/* tensors of the whole tiles, then of the rests */
+	std::vector<uint32_t> rest;
 	std::vector<void *> grads((size_t)n);
 	uint64_t tiles = 0;
 	uint64_t block0 = 0;
@@ -850,6 +922,7 @@ static int create(const anni_mt_tensor *list, int n, anni_mtstep *h)
 	int per_sm = 0;
 	int rc;
 
+	h->aligned = true;
 	for (int i = 0; i < n; i++) {
 		rc = check_tensor(&list[i], h->state_dtype, h->written);
 		if (rc != ANNI_OK)
@@ -858,11 +931,14 @@ static int create(const anni_mt_tensor *list, int n, anni_mtstep *h)
 		grads[i] = list[i].grad;
 		desc[i] = { list[i].param, list[i].m, list[i].v, list[i].m_scale, list[i].v_scale,
 		    (list[i].flags & ANNI_SEG_TWIN_BF16) ? (uint16_t *)list[i].twin_bf16 : NULL, list[i].n, block0,
-		    (uint32_t)tiles, (uint16_t)((list[i].flags & ANNI_SEG_WD) ? 1 : 0), 0 };
-		desc[i].vec = aligned(desc[i], h->state_dtype == ANNI_DT_Q8);
-		tiles += (uint64_t)(list[i].n + ANNI_MT_TILE - 1) / ANNI_MT_TILE;
+		    (uint32_t)tiles, (list[i].flags & ANNI_SEG_WD) ? 1u : 0u };
+		if (list[i].n > 0 && !aligned(desc[i], h->state_dtype == ANNI_DT_Q8))
+			h->aligned = false;
+		tiles += (uint64_t)list[i].n / ANNI_MT_TILE;
 		block0 += (uint64_t)(list[i].n + ANNI_MT_BLOCK - 1) / ANNI_MT_BLOCK;
-		if (tiles > 0x7fffffffu)
+		if (list[i].n % ANNI_MT_TILE)
+			rest.push_back((uint32_t)i);
+		if (tiles + rest.size() > 0x7fffffffu)
 			return ANNI_E_LIMIT;
 	}
 	std::sort(h->written.begin(), h->written.end());
@@ -871,28 +947,32 @@ static int create(const anni_mt_tensor *list, int n, anni_mtstep *h)
 	rc = check_grads(h, grads.data());
 	if (rc != ANNI_OK)
 		return rc;
-	tile_of.reserve((size_t)tiles);
+	table.reserve((size_t)tiles + rest.size() + 1);
 	for (int i = 0; i < n; i++)
-		tile_of.insert(tile_of.end(), (size_t)((list[i].n + ANNI_MT_TILE - 1) / ANNI_MT_TILE), (uint32_t)i);
+		table.insert(table.end(), (size_t)(list[i].n / ANNI_MT_TILE), (uint32_t)i);
+	table.insert(table.end(), rest.begin(), rest.end());
 	h->tiles = (uint32_t)tiles;
+	h->rests = (uint32_t)rest.size();
 	if (cudaGetDevice(&h->device) != cudaSuccess
-	    || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, h->device) != cudaSuccess
-	    || cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, step_kernel(h->grad_dtype, h->state_dtype),
-	    ANNI_THREADS, 0) != cudaSuccess || sms < 1 || per_sm < 1
+	    || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, h->device) != cudaSuccess || sms < 1
 	    || cudaMalloc((void **)&h->ctl, sizeof(anni_control)) != cudaSuccess
 	    || cudaMalloc((void **)&h->desc, (size_t)n * sizeof(mt_desc)) != cudaSuccess
 	    || cudaMalloc((void **)&h->grad, (size_t)n * sizeof(void *)) != cudaSuccess
-	    || cudaMalloc((void **)&h->tile_of, ((size_t)tiles + 1) * sizeof(uint32_t)) != cudaSuccess
+	    || cudaMalloc((void **)&h->tile_of, (table.size() + 1) * sizeof(uint32_t)) != cudaSuccess
 	    || cudaMemset(h->ctl, 0, sizeof(anni_control)) != cudaSuccess
 	    || cudaMemcpy(h->desc, desc.data(), (size_t)n * sizeof(mt_desc), cudaMemcpyHostToDevice) != cudaSuccess
 	    || cudaMemcpy(h->grad, grads.data(), (size_t)n * sizeof(void *), cudaMemcpyHostToDevice) != cudaSuccess
-	    || cudaMemcpy(h->tile_of, tile_of.data(), (size_t)tiles * sizeof(uint32_t), cudaMemcpyHostToDevice)
-	    != cudaSuccess) {
+	    || cudaMemcpy(h->tile_of, table.data(), table.size() * sizeof(uint32_t), cudaMemcpyHostToDevice) != cudaSuccess) {
+		(void)cudaGetLastError();
+		return ANNI_E_CUDA;
+	}
+	if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, step_kernel(h->grad_dtype, h->state_dtype, h->aligned),
+	    ANNI_THREADS, 0) != cudaSuccess || per_sm < 1) {
 		(void)cudaGetLastError();
 		return ANNI_E_CUDA;
 	}
 	h->blocks = std::min(sms * per_sm, ANNI_MAX_BLOCKS / sms * sms);
-	h->blocks = (int)std::max((uint64_t)1, std::min((uint64_t)h->blocks, tiles));
+	h->blocks = (int)std::max((uint64_t)1, std::min((uint64_t)h->blocks, tiles + rest.size()));
 	return ANNI_OK;
 }
 
@@ -976,7 +1056,9 @@ extern "C" int anni_mtstep_step(anni_mtstep *h, const anni_optstep_hyper *hp, ui
 	a.desc = h->desc;
 	a.grad = h->grad;
 	a.tile_of = h->tile_of;
+	a.rest_of = h->tile_of + h->tiles;
 	a.tiles = h->tiles;
+	a.rests = h->rests;
 	a.seed = seed;
 	a.b1 = (float)a.la.b1;
 	a.omb1 = (float)a.la.omb1;
@@ -989,7 +1071,8 @@ extern "C" int anni_mtstep_step(anni_mtstep *h, const anni_optstep_hyper *hp, ui
 	{
 		const int slot = anni_op_begin(ANNI_OP_ADAM, stream);
 
-		rc = cudaLaunchCooperativeKernel(step_kernel(h->grad_dtype, h->state_dtype), dim3(h->blocks),
+
+		rc = cudaLaunchCooperativeKernel(step_kernel(h->grad_dtype, h->state_dtype, h->aligned), dim3(h->blocks),
 		    dim3(ANNI_THREADS), args, 0, (cudaStream_t)stream) == cudaSuccess ? ANNI_OK : ANNI_E_CUDA;
 		anni_op_end(slot, stream);
 	}

@@ -6,10 +6,10 @@ Error bounds.  u = 2^-24 is half a step of float, relative to the value.
   of the old and the new value and 1e-6 of the change (SFU square root and reciprocal, two products).
 * 8-bit moments are computed in float: the stored value code * scale, beta, 1 - beta, the clip factor and the
   gradient's product with it are each rounded once (u), the product of the second term (for v: two) once, and
-  their sum once: at most 8 u of |b1 m| + |(1 - b1) g|, resp. of b2 v + (1 - b2) g^2.  The scale adds a
-  division and inherits the error of the largest element: 9 u of the largest such sum in the block.  A value
-  over its scale, y, then carries those 8 u of its terms, those 9 u of y, one product and one quotient: DELTA
-  below.  The stored number must be as near to the exact y as the nearest one, but for 2 DELTA.
+  their sum once: at most 8 u of |b1 m| + |(1 - b1) g|, resp. of b2 v + (1 - b2) g^2.  The scale inherits the
+  error of the largest element and adds a constant's and a product's: 10 u of the largest such sum in the block.  A
+  value over its scale, y, carries those 8 u of its terms, 8 u of the largest element's, and the roundings of a
+  reciprocal and two products: at most DELTA below.  The stored number must be as near to the exact y as the nearest one, but for 2 DELTA.
 """
 import ctypes as C
 import math
@@ -295,6 +295,29 @@ def test_8_bit_edges():
 
 
 @gpu
+@pytest.mark.parametrize("stochastic", [False, True])
+def test_8_bit_codes_are_those_of_the_float_formula(stochastic):
+    """Every product and sum is rounded on its own: the formula in torch's fp32 gives the same codes and scales."""
+    n = 256 * 400
+    c = Case([n], DT_F32, DT_Q8, seed=21, twin=False)
+    m0, v0, ms0, vs0, g = (x[0].clone() for x in (c.m, c.v, c.ms, c.vs, c.g))
+    c.step.step(hyper(check=False, stochastic=stochastic), seed=77)
+    at = lambda codes, scale: codes.float().view(-1, 256) * scale.view(-1, 1)  # noqa: E731
+    b1, b2 = HYP["beta1"], HYP["beta2"]
+    g = g.view(-1, 256)
+    m = b1 * at(m0, ms0) + (1 - b1) * g
+    v = b2 * at(v0, vs0) + (1 - b2) * g * g
+    for x, codes, scale, top in ((m, c.m[0], c.ms[0], 448.0), (v, c.v[0], c.vs[0], 57344.0)):
+        amax = x.abs().amax(1, keepdim=True)
+        assert torch.equal(scale, (amax / top).view(-1))
+        if not stochastic:
+            want = (x * (top / amax)).clamp(-top, top).to(codes.dtype)
+            if top > 448:
+                want = torch.maximum(want.view(torch.uint8), (x > 0).to(torch.uint8)).view(codes.dtype)
+            assert torch.equal(codes.view(torch.uint8), want.view(-1).view(torch.uint8))
+
+
+@gpu
 def test_stochastic_rounding_is_unbiased():
     """v decays by 0.1 % a step; to nearest it stays where it is, stochastically it follows on average.
 
@@ -351,6 +374,28 @@ def test_captured_and_replayed(state_dtype):
         got = x.snapshot()
         for k in ("p", "m", "v", "twin"):
             assert all(torch.equal(y.contiguous().view(torch.uint8), z.contiguous().view(torch.uint8)) for y, z in zip(got[k], want[k])), k
+
+
+@gpu
+@pytest.mark.parametrize("state_dtype", [DT_F32, DT_Q8])
+def test_gradients_move_between_replays(state_dtype):
+    """A captured step takes the addresses that the handle has when it is replayed, on the 16-byte grid or off it."""
+    c = Case([300, 5000, 70001, 2048], DT_BF16, state_dtype, seed=13)
+    gr, st = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(gr, stream=st):
+        c.step.step(hyper(0.5, zero=True))
+    room = [torch.zeros(g.numel() + 3, dtype=g.dtype, device="cuda") for g in c.g]
+    moved = [r[1 + k % 3:][:g.numel()] for k, (r, g) in enumerate(zip(room, c.g))]
+    for a, b in zip(moved, c.g):
+        a.copy_(b)
+    c.step.set_grads(moved)
+    torch.cuda.synchronize()
+    gr.replay()
+    torch.cuda.synchronize()
+    kept = c.snapshot()["g"]
+    assert all(torch.equal(a, b) for a, b in zip(kept, c.before["g"])) and not any(r.any() for r in room)
+    c.check(HYP, clip=0.5)
 
 
 @gpu
