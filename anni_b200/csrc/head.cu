@@ -1,13 +1,13 @@
 /*
 ** Loss and gradients of a language model's head (include/anni_head.h).
 **
-** Four matrix products on the tensor cores, one persistent kernel each:
+** Four matrix products on the tensor cores, in three persistent kernels:
 **   loss    logits of a tile of rows and vocabulary; its epilogue keeps the maximum and the sum of exponentials
 **           of each row and drops the logits.  A small kernel joins the tiles of a row.
 **   delta   the same logits again for one piece of the vocabulary; softmax - one-hot from lse, stored as bf16
 **           (three terms of it for fp32 gradients), and its column sums for dbias
-**   dx      delta W^T of the piece, added to an fp32 sum over the pieces
-**   dw      x^T delta of the piece, stored or added to the gradient
+**   grad    dx = delta W^T of the piece, added to an fp32 sum over the pieces, and dw = x^T delta of the piece, stored
+**           or added to the gradient; together, so that the tiles of one fill the rounds that the other leaves open
 ** Bound by the tensor cores: 2 T D V operations each (the logits twice, since they are not kept).
 **
 ** Two blocks (a cluster on two neighbouring SMs) work on a 256 x 256 tile: each keeps 128 rows of the result
@@ -56,7 +56,8 @@
 
 namespace {
 
-enum { LOSS, DELTA, DX, DW };
+enum { LOSS, DELTA, GRAD };
+enum { DX, DW };	/* the products of GRAD */
 
 struct head_args {
 	const __nv_bfloat16	*x;
@@ -93,14 +94,22 @@ struct head_args {
 	int			add;
 };
 
-struct gemm_args {
+/* one product: operands, tiles, and how its sums are cut */
+struct product_args {
 	CUtensorMap	a;
 	CUtensorMap	b;
-	head_args	h;
 	int		m_tiles;
 	int		n_tiles;
 	int		k_blocks;	/* of one term */
 	int		run;		/* ... of them that one accumulator adds up */
+	int		total;		/* tiles, times the parts of dx */
+};
+
+struct gemm_args {
+	product_args	p[2];		/* GRAD: dx and dw; otherwise the first alone */
+	head_args	h;
+	int		first;		/* GRAD: the product with the longer tiles, which go first */
+	int		extra;		/* tiles of the other that a pair with one fewer of those gets for it */
 };
 
 /* ---- PTX ------------------------------------------------------------------------------------------ */
@@ -279,6 +288,7 @@ __device__ __forceinline__ float to_f(__nv_bfloat16 v)
 /* ---- which tile, and what of it a stage holds ---------------------------------------------------- */
 
 struct tile_at {
+	int	which;	/* GRAD: DX or DW */
 	int	m0;	/* this block's rows */
 	int	n0;
 	int	b0;	/* its share of the second operand */
@@ -287,64 +297,101 @@ struct tile_at {
 	int	split;
 };
 
+/* how many of 0 .. n - 1 are at + i * step */
+__device__ __forceinline__ int count_of(int n, int at, int step)
+{
+	return at < n ? (n - at + step - 1) / step : 0;
+}
+
 /*
-** Order of the tiles.  loss, delta: all row tiles (32 at most) of one column tile after another, so that W is
-** read once while x stays in L2; dx: the column tiles of a row tile together, dw: the row tiles of a column tile
-** together, so that delta is read once.
+** The i-th tile of a pair of blocks; false: there is none.
+**
+** loss, delta: all row tiles (32 at most) of one column tile after another, dealt round-robin, so that W is read
+** once while x stays in L2.  grad: the longer tiles round-robin; the pairs that get one fewer of them take `extra`
+** of the shorter ones for it, the rest of those go round-robin again.  Within dx the column tiles of a row
+** tile come together, within dw the row tiles of a column tile, so that delta is read once.
 */
 template <int KIND>
-__device__ __forceinline__ tile_at tile_of(const gemm_args &g, int t, int rank)
+__device__ __forceinline__ bool tile_of(const gemm_args &g, int i, int rank, int pair, int pairs, tile_at &r)
 {
-	tile_at r;
+	int t;
 	int m;
 	int n;
 
 	r.split = 0;
-	r.k0 = 0;
-	r.k1 = g.k_blocks;
-	if (KIND == DX) {
-		n = t % g.n_tiles;
-		m = t / g.n_tiles % g.m_tiles;
-		r.split = t / (g.n_tiles * g.m_tiles);
-		r.k0 = (int)((int64_t)g.k_blocks * r.split / g.h.splits);
-		r.k1 = (int)((int64_t)g.k_blocks * (r.split + 1) / g.h.splits);
-	} else if (KIND == DW) {
-		m = t % g.m_tiles;
-		n = t / g.m_tiles;
-	} else {
-		const int group = t / (32 * g.n_tiles);
-		const int rows = min(32, g.m_tiles - group * 32);
-		const int i = t - group * 32 * g.n_tiles;
+	r.which = 0;
+	if (KIND == GRAD) {
+		const int n_long = g.p[g.first].total;
+		const int n_short = g.p[1 - g.first].total;
+		const int own = count_of(n_long, pair, pairs);
+		const int full = n_long % pairs;		/* pairs with one more */
+		const int lack = pairs - full;
+		const int fill = min(n_short, lack * g.extra);
+		const int own_fill = pair >= full ? count_of(fill, pair - full, lack) : 0;
 
-		m = group * 32 + i % rows;
-		n = i / rows;
+		if (i < own) {
+			r.which = g.first;
+			t = pair + i * pairs;
+		} else {
+			i -= own;
+			r.which = 1 - g.first;
+			t = i < own_fill ? pair - full + i * lack : fill + (pair + lack) % pairs + (i - own_fill) * pairs;
+			if (t >= n_short)
+				return false;
+		}
+	} else {
+		t = pair + i * pairs;
+		if (t >= g.p[0].total)
+			return false;
+	}
+	const product_args &p = g.p[r.which];
+
+	r.k0 = 0;
+	r.k1 = p.k_blocks;
+	if (KIND == GRAD && r.which == DX) {
+		n = t % p.n_tiles;
+		m = t / p.n_tiles % p.m_tiles;
+		r.split = t / (p.n_tiles * p.m_tiles);
+		r.k0 = (int)((int64_t)p.k_blocks * r.split / g.h.splits);
+		r.k1 = (int)((int64_t)p.k_blocks * (r.split + 1) / g.h.splits);
+	} else if (KIND == GRAD) {
+		m = t % p.m_tiles;
+		n = t / p.m_tiles;
+	} else {
+		const int group = t / (32 * p.n_tiles);
+		const int rows = min(32, p.m_tiles - group * 32);
+
+		t -= group * 32 * p.n_tiles;
+		m = group * 32 + t % rows;
+		n = t / rows;
 	}
 	r.m0 = m * HEAD_TM + rank * HEAD_HALF;
 	r.n0 = n * HEAD_TN;
 	r.b0 = r.n0 + rank * HEAD_HALF;
-	return r;
+	return true;
 }
 
 template <int KIND>
 __device__ __forceinline__ void load_stage(const gemm_args &g, const tile_at &t, int term, int k, uint32_t dst, uint32_t bar)
 {
+	const product_args &p = g.p[t.which];
 	const uint32_t b = dst + HEAD_A_BYTES;
 
-	if (KIND == LOSS || KIND == DELTA) {
-		tma_load(dst, &g.a, bar, k, t.m0, 0);
+	if (KIND != GRAD) {
+		tma_load(dst, &p.a, bar, k, t.m0, 0);
 #pragma unroll
 		for (int j = 0; j < HEAD_HALF / 64; j++)
-			tma_load(b + j * HEAD_MN_BYTES, &g.b, bar, g.h.v0 + t.b0 + 64 * j, k, 0);
-	} else if (KIND == DX) {
-		tma_load(dst, &g.a, bar, k, t.m0, term);
-		tma_load(b, &g.b, bar, g.h.v0 + k, t.b0, 0);
+			tma_load(b + j * HEAD_MN_BYTES, &p.b, bar, g.h.v0 + t.b0 + 64 * j, k, 0);
+	} else if (t.which == DX) {
+		tma_load(dst, &p.a, bar, k, t.m0, term);
+		tma_load(b, &p.b, bar, g.h.v0 + k, t.b0, 0);
 	} else {
 #pragma unroll
 		for (int j = 0; j < HEAD_HALF / 64; j++)
-			tma_load(dst + j * HEAD_MN_BYTES, &g.a, bar, t.m0 + 64 * j, k, 0);
+			tma_load(dst + j * HEAD_MN_BYTES, &p.a, bar, t.m0 + 64 * j, k, 0);
 #pragma unroll
 		for (int j = 0; j < HEAD_HALF / 64; j++)
-			tma_load(b + j * HEAD_MN_BYTES, &g.b, bar, t.b0 + 64 * j, k, term);
+			tma_load(b + j * HEAD_MN_BYTES, &p.b, bar, t.b0 + 64 * j, k, term);
 	}
 }
 
@@ -563,84 +610,132 @@ __device__ __forceinline__ float2 unpack2(uint32_t q)
 	return make_float2(__uint_as_float(q << 16), __uint_as_float(q & 0xffff0000u));
 }
 
+/* 32 x 32 values of a warp, lane l with row l, so that lane l has column l: v[i] is then of row i */
+__device__ __forceinline__ void transpose(float (&v)[32])
+{
+	const int lane = threadIdx.x & 31;
+
+#pragma unroll
+	for (int s = 16; s > 0; s >>= 1)
+#pragma unroll
+		for (int i = 0; i < 32; i++)
+			if (!(i & s)) {
+				const bool up = lane & s;
+				const float got = __shfl_xor_sync(0xffffffffu, up ? v[i] : v[i + s], s);
+
+				if (up)
+					v[i] = got;
+				else
+					v[i + s] = got;
+			}
+}
+
 /*
-** Eight or sixteen consecutive results (32 bytes) of a row, stored or added to what is there, element by element where
-** the row ends or its address is not on 32 bytes.
+** A warp's 32 x 32 results, lane l with row l, stored or added to what is there: at (row, col) of a matrix of which
+** `rows` rows and `left` of these columns exist.  Rows on 32 bytes: every lane whole sectors of its own row; others:
+** transposed, the warp row by row, so that its accesses are one piece whatever the address.
 */
-template <typename T, int N>
-__device__ __forceinline__ void put_some(T *out, const float *v, int left, bool add)
+__device__ __forceinline__ void put_block(void *base, int64_t ld, int row, int rows, int64_t col, int left, float (&v)[32],
+	bool bf16, bool add)
 {
-	if (left >= N && ((uintptr_t)out & 31) == 0) {
-		uint32_t r[8] = { 0, 0, 0, 0, 0, 0, 0, 0 };
+	const int lane = threadIdx.x & 31;
+	const int size = bf16 ? 2 : 4;
 
-		if (add)
-			load32(out, r);
+	if (left >= 32 && (((uintptr_t)base | (uintptr_t)(ld * size) | (uintptr_t)(col * size)) & 31) == 0) {
+		char *out = static_cast<char *>(base) + ((int64_t)(row + lane) * ld + col) * size;
+
+		if (row + lane >= rows)
+			return;
+		if (bf16) {
 #pragma unroll
-		for (int j = 0; j < 8; j++)
-			if (N == 16) {
-				const float2 q = unpack2(r[j]);
+			for (int i = 0; i < 32; i += 16) {
+				uint32_t r[8] = { 0, 0, 0, 0, 0, 0, 0, 0 };
 
-				r[j] = bf16_pair(q.x + v[2 * j % N], q.y + v[(2 * j + 1) % N]);
-			} else
-				r[j] = __float_as_uint(__uint_as_float(r[j]) + v[j]);
-		store32(out, r);
+				if (add)
+					load32(out + i * 2, r);
+#pragma unroll
+				for (int j = 0; j < 8; j++) {
+					const float2 q = unpack2(r[j]);
+
+					r[j] = bf16_pair(q.x + v[i + 2 * j], q.y + v[i + 2 * j + 1]);
+				}
+				store32(out + i * 2, r);
+			}
+		} else {
+#pragma unroll
+			for (int i = 0; i < 32; i += 8) {
+				uint32_t r[8] = { 0, 0, 0, 0, 0, 0, 0, 0 };
+
+				if (add)
+					load32(out + i * 4, r);
+#pragma unroll
+				for (int j = 0; j < 8; j++)
+					r[j] = __float_as_uint(__uint_as_float(r[j]) + v[i + j]);
+				store32(out + i * 4, r);
+			}
+		}
 		return;
 	}
-#pragma unroll
-	for (int j = 0; j < N; j++)
-		if (j < left)
-			put(out, j, v[j], N == 16, add);
-}
-
-/* 32 columns of a row of a matrix of the gradients' type, `left` of which exist */
-__device__ __forceinline__ void put_row(void *base, int64_t first, const float (&v)[32], int left, bool bf16, bool add)
-{
+	transpose(v);
+	if (lane >= left)
+		return;
 	if (bf16) {
+		__nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(base) + (int64_t)row * ld + col + lane;
+
 #pragma unroll
-		for (int i = 0; i < 32; i += 16)
-			put_some<__nv_bfloat16, 16>(static_cast<__nv_bfloat16 *>(base) + first + i, v + i, left - i, add);
+		for (int i = 0; i < 32; i += 4) {
+			float old[4];
+
+#pragma unroll
+			for (int j = 0; j < 4; j++)
+				old[j] = add && row + i + j < rows ? to_f(out[j * ld]) : 0.0f;
+#pragma unroll
+			for (int j = 0; j < 4; j++)
+				if (row + i + j < rows)
+					out[j * ld] = __float2bfloat16_rn(old[j] + v[i + j]);
+			out += 4 * ld;
+			asm volatile("" ::: "memory");
+		}
 	} else {
+		float *out = static_cast<float *>(base) + (int64_t)row * ld + col + lane;
+
 #pragma unroll
-		for (int i = 0; i < 32; i += 8)
-			put_some<float, 8>(static_cast<float *>(base) + first + i, v + i, left - i, add);
+		for (int i = 0; i < 32; i += 4) {
+			float old[4];
+
+#pragma unroll
+			for (int j = 0; j < 4; j++)
+				old[j] = add && row + i + j < rows ? out[j * ld] : 0.0f;
+#pragma unroll
+			for (int j = 0; j < 4; j++)
+				if (row + i + j < rows)
+					out[j * ld] = old[j] + v[i + j];
+			out += 4 * ld;
+			asm volatile("" ::: "memory");
+		}
 	}
 }
 
-__device__ __forceinline__ void dx_epilogue(const gemm_args &g, const tile_at &at, float (&acc)[4][32])
+__device__ __forceinline__ void grad_epilogue(const gemm_args &g, const tile_at &at, float (&acc)[4][32])
 {
 	const head_args &h = g.h;
-	const int t = at.m0 + epi_row();
+	const int row = at.m0 + (epi_row() & ~31);	/* this warp's first */
+	const bool dx = at.which == DX;
+	const bool parts = dx && h.dxp;
+	/* dx: its fp32 sum, or where one part of one piece is all of it, dx itself */
+	void *const base = parts ? h.dxp + (int64_t)at.split * h.tokens * h.ldd : dx ? h.dx : h.dw;
+	const int64_t ld = parts ? h.ldd : dx ? h.lddx : h.lddw;
+	const int rows = dx ? h.tokens : h.d;
+	const int cols = parts ? h.ldd : dx ? h.d : h.v1;
+	const bool add = parts ? h.v0 != 0 : !dx && h.add;
+	const int col = (dx ? 0 : h.v0) + at.n0 + epi_col();
 
-	if (t >= h.tokens)
-		return;
 #pragma unroll
-	for (int c = 0; c < 4; c++) {
-		const int d = at.n0 + epi_col() + c * 32;
-
-		if (d >= h.d)
-			break;
-		if (h.dxp)
-			put_row(h.dxp, ((int64_t)at.split * h.tokens + t) * h.ldd + d, acc[c], h.ldd - d, false, h.v0 != 0);
-		else		/* one part, one piece: that is dx */
-			put_row(h.dx, t * h.lddx + d, acc[c], h.d - d, h.bf16, false);
-	}
-}
-
-__device__ __forceinline__ void dw_epilogue(const gemm_args &g, const tile_at &at, float (&acc)[4][32])
-{
-	const head_args &h = g.h;
-	const int d = at.m0 + epi_row();
-
-	if (d >= h.d)
-		return;
-#pragma unroll
-	for (int c = 0; c < 4; c++) {
-		const int v = h.v0 + at.n0 + epi_col() + c * 32;
-
-		if (v >= h.v1)
-			break;
-		put_row(h.dw, (int64_t)d * h.lddw + v, acc[c], h.v1 - v, h.bf16, h.add);
-	}
+	for (int c = 0; c < 4; c++)
+		if (col + c * 32 < cols && row < rows) {
+			put_block(base, ld, row, rows, col + c * 32, cols - col - c * 32, acc[c], h.bf16 && !parts, add);
+			asm volatile("" ::: "memory");	/* one 32 after the other: what is read ahead is spilled */
+		}
 }
 
 /* ---- the product -------------------------------------------------------------------------------------- */
@@ -661,14 +756,14 @@ struct gemm_smem {
 ** are issued there.  Returns after a give-up only when the copies in flight have landed, or the time is up.
 */
 template <int KIND>
-__device__ __forceinline__ void producer(const gemm_args &g, gemm_smem *s, uint32_t ring, int total, int rank, int pair, int pairs)
+__device__ __forceinline__ void producer(const gemm_args &g, gemm_smem *s, uint32_t ring, int rank, int pair, int pairs)
 {
-	const int terms = KIND == DX || KIND == DW ? g.h.terms : 1;
+	const int terms = KIND == GRAD ? g.h.terms : 1;
 	uint32_t n = 0;		/* stages loaded so far */
+	tile_at at;
 
-	for (int tile = pair; tile < total; tile += pairs) {
-		const tile_at at = tile_of<KIND>(g, tile, rank);
-
+	for (int tile = 0; tile_of<KIND>(g, tile, rank, pair, pairs, at); tile++) {
+		const int run = g.p[at.which].run;
 		int k = at.k0;
 		int term = 0;
 		int from = k;	/* of this run */
@@ -693,7 +788,7 @@ __device__ __forceinline__ void producer(const gemm_args &g, gemm_smem *s, uint3
 			load_stage<KIND>(g, at, terms - 1 - term, k * HEAD_TK, ring + i * HEAD_STAGE_BYTES,
 			    smem_in(smem_of(&s->full[i]), 0));
 			n++;
-			if (++k == min(from + g.run, at.k1)) {
+			if (++k == min(from + run, at.k1)) {
 				if (++term == terms) {
 					term = 0;
 					from = k;
@@ -706,19 +801,23 @@ __device__ __forceinline__ void producer(const gemm_args &g, gemm_smem *s, uint3
 
 /* the first block's: issues the products of both */
 template <int KIND>
-__device__ __forceinline__ void multiplier(const gemm_args &g, gemm_smem *s, uint32_t ring, int total, int pair, int pairs)
+__device__ __forceinline__ void multiplier(const gemm_args &g, gemm_smem *s, uint32_t ring, int pair, int pairs)
 {
-	const bool a_mn = KIND == DW;
-	const bool b_mn = KIND != DX;
-	const uint32_t idesc = instr_desc(a_mn, b_mn);
 	uint32_t n = 0;
 	uint32_t done = 0;	/* runs */
+	tile_at at;
 
-	for (int tile = pair; tile < total; tile += pairs) {
-		const tile_at at = tile_of<KIND>(g, tile, 0);
+	for (int tile = 0; tile_of<KIND>(g, tile, 0, pair, pairs, at); tile++) {
+		const bool a_mn = KIND == GRAD && at.which == DW;
+		const bool b_mn = KIND != GRAD || at.which == DW;
+		const uint32_t idesc = instr_desc(a_mn, b_mn);
+		/* 16 k a time: 32 bytes further in a K-major row, 16 rows of 128 bytes further in an MN-major box */
+		const uint32_t a_step = a_mn ? 2048 : 32;
+		const uint32_t b_step = b_mn ? 2048 : 32;
+		const int run = g.p[at.which].run;
 
-		for (int from = at.k0; from < at.k1; from += g.run, done++) {
-			const int steps = (min(from + g.run, at.k1) - from) * (KIND == DX || KIND == DW ? g.h.terms : 1);
+		for (int from = at.k0; from < at.k1; from += run, done++) {
+			const int steps = (min(from + run, at.k1) - from) * (KIND == GRAD ? g.h.terms : 1);
 			const uint32_t acc = s->tmem + (done & 1) * HEAD_TN;
 			bool ok = mbar_wait(smem_of(&s->drained[done & 1]), (done / 2 & 1) ^ 1, &s->stop);
 
@@ -731,14 +830,10 @@ __device__ __forceinline__ void multiplier(const gemm_args &g, gemm_smem *s, uin
 				if (!ok)
 					break;
 				asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-				/*
-				** 16 k a time: 32 bytes further in a K-major row, 16 rows of 128 bytes further in an
-				** MN-major box
-				*/
 #pragma unroll
 				for (int j = 0; j < HEAD_TK / 16; j++)
-					mma(acc, smem_desc(base + j * (a_mn ? 2048 : 32), a_mn),
-					    smem_desc(base + HEAD_A_BYTES + j * (b_mn ? 2048 : 32), b_mn), idesc, k > 0 || j > 0);
+					mma(acc, smem_desc(base + j * a_step, a_mn),
+					    smem_desc(base + HEAD_A_BYTES + j * b_step, b_mn), idesc, k > 0 || j > 0);
 				mma_commit(smem_of(&s->empty[i]));
 			}
 			if (!ok) {
@@ -752,14 +847,15 @@ __device__ __forceinline__ void multiplier(const gemm_args &g, gemm_smem *s, uin
 }
 
 template <int KIND>
-__device__ __forceinline__ void drainer(const gemm_args &g, gemm_smem *s, int total, int rank, int pair, int pairs)
+__device__ __forceinline__ void drainer(const gemm_args &g, gemm_smem *s, int rank, int pair, int pairs)
 {
 	const uint32_t lanes = (uint32_t)(threadIdx.x >> 5 & 3) << 21;	/* this warp's quarter of the lanes: 32 w << 16 */
 	uint32_t done = 0;
 	uint32_t b = 0;
+	tile_at at;
 
-	for (int tile = pair; tile < total; tile += pairs, b ^= 1) {
-		const tile_at at = tile_of<KIND>(g, tile, rank);
+	for (int tile = 0; tile_of<KIND>(g, tile, rank, pair, pairs, at); tile++, b ^= 1) {
+		const int run = g.p[at.which].run;
 		float acc[4][32];
 
 		if (KIND == LOSS)
@@ -767,7 +863,7 @@ __device__ __forceinline__ void drainer(const gemm_args &g, gemm_smem *s, int to
 		if (KIND == DELTA)
 			stage_bias(g.h, g.h.v0 + at.n0, g.h.v1, s->epi.bias[b]);
 #pragma unroll 1
-		for (int from = at.k0; from < at.k1; from += g.run, done++) {
+		for (int from = at.k0; from < at.k1; from += run, done++) {
 			const uint32_t addr = s->tmem + lanes + (done & 1) * HEAD_TN + epi_col();
 
 			/* the warps keep step with each other even after a give-up, for the barriers' sake */
@@ -806,10 +902,8 @@ __device__ __forceinline__ void drainer(const gemm_args &g, gemm_smem *s, int to
 			loss_epilogue(g, at, acc, s->epi.bias[b], s->epi.half[b]);
 		else if (KIND == DELTA)
 			delta_epilogue(g, at, acc, s->epi.bias[b], s->epi.sums[b]);
-		else if (KIND == DX)
-			dx_epilogue(g, at, acc);
 		else
-			dw_epilogue(g, at, acc);
+			grad_epilogue(g, at, acc);
 	}
 }
 
@@ -834,7 +928,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HEAD_THREADS, 1) pro
 	const int rank = blockIdx.x & 1;
 	const int pair = blockIdx.x >> 1;
 	const int pairs = gridDim.x >> 1;
-	const int total = g.m_tiles * g.n_tiles * (KIND == DX ? g.h.splits : 1);
 
 	if (threadIdx.x == 0) {
 		for (int i = 0; i < HEAD_STAGES; i++) {
@@ -862,11 +955,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HEAD_THREADS, 1) pro
 	dependent();
 	if (warp < 4) {
 		if (warp == 0 && (threadIdx.x & 31) == 0)
-			producer<KIND>(g, &s, ring, total, rank, pair, pairs);
+			producer<KIND>(g, &s, ring, rank, pair, pairs);
 		if (warp == 1 && (threadIdx.x & 31) == 0 && rank == 0)
-			multiplier<KIND>(g, &s, ring, total, pair, pairs);
+			multiplier<KIND>(g, &s, ring, pair, pairs);
 	} else
-		drainer<KIND>(g, &s, total, rank, pair, pairs);
+		drainer<KIND>(g, &s, rank, pair, pairs);
 	__syncwarp();
 	asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 	__syncthreads();
@@ -1207,25 +1300,64 @@ size_t take(size_t *at, int64_t bytes)
 	return here;
 }
 
-/*
-** Into how many parts the sum over the vocabulary in dx is cut: the number of tiles of dx does not depend on the
-** vocabulary, and often leaves pairs of SMs idle in the last round.  The fewest parts, of at least eight stages,
-** whose rounds waste the least.  (4096 rows of 1536: 96 tiles are two rounds of 74 pairs, 65 % used; three parts
-** make four shorter rounds, 97 %.)
-*/
-int split_dx(int64_t tiles_of_dx, int64_t stages)
+/* tiles of the two products of the gradients over one piece of `width` columns, and stages of a tile (all terms) */
+struct grad_work {
+	int64_t	tiles[2];
+	int64_t	stages[2];
+};
+
+grad_work work_of(int64_t tokens, int64_t d, int64_t width, int terms, bool dx, bool dw, int splits)
 {
+	grad_work w;
+
+	w.tiles[DX] = dx ? up(tokens, HEAD_TM) / HEAD_TM * (up(d, HEAD_TN) / HEAD_TN) * splits : 0;
+	w.tiles[DW] = dw ? up(d, HEAD_TM) / HEAD_TM * (up(width, HEAD_TN) / HEAD_TN) : 0;
+	w.stages[DX] = (up(width, HEAD_TK) / HEAD_TK * terms + splits - 1) / splits;
+	w.stages[DW] = up(tokens, HEAD_TK) / HEAD_TK * terms;
+	return w;
+}
+
+/* which product goes first, and how many tiles of the other make up for one of it */
+void order(const grad_work &w, int *first, int *extra)
+{
+	*first = w.stages[DX] >= w.stages[DW] ? DX : DW;
+	*extra = (int)((w.stages[*first] + w.stages[1 - *first] / 2) / w.stages[1 - *first]);
+}
+
+/*
+** Into how many parts the sum over the vocabulary in dx is cut: as many as make the busiest pair of SMs finish
+** first.  A stage takes a pair 512 cycles (0.27 us); every part is written and read once more as fp32, at 6.5 TB/s.
+** With dw's tiles to fill the rounds one part is best for many rows; a few rows have few tiles of dx, whose sums
+** are as long as the vocabulary (128 rows of 1536 against 100,000 entries: 6 tiles of 1563 stages).
+*/
+int split_dx(int64_t tokens, int64_t d, int64_t width, int terms, bool dw)
+{
+	const int64_t stages = up(width, HEAD_TK) / HEAD_TK;
 	int best = 1;
-	double least = 1e30;
+	double least = 0.0;
 
-	for (int s = 1; s <= HEAD_PAIRS && (s == 1 || stages / s >= 8); s++) {
-		const double rounds = (double)up(tiles_of_dx * s, HEAD_PAIRS) / HEAD_PAIRS / s;
+	for (int n = 1; n <= HEAD_PAIRS && (n == 1 || stages / n >= 4); n++) {
+		const grad_work w = work_of(tokens, d, width, terms, true, dw, n);
+		int first;
+		int extra;
+		int64_t full;
+		int64_t fill;
+		int64_t most;
+		int64_t least_long;
+		double time;
 
-		if (s > 4 && tiles_of_dx >= HEAD_PAIRS)
-			break;		/* each part costs a pass over an fp32 copy of dx */
-		if (rounds < least * 0.97) {
-			least = rounds;
-			best = s;
+		order(w, &first, &extra);
+		full = w.tiles[first] % HEAD_PAIRS;
+		least_long = w.tiles[first] / HEAD_PAIRS * w.stages[first];
+		fill = std::min(w.tiles[1 - first], (HEAD_PAIRS - full) * extra);
+		/* pairs with one more of the long tiles, and those that got short ones for it; then the rest for all */
+		most = std::max(full ? least_long + w.stages[first] : 0,
+		    least_long + (fill + HEAD_PAIRS - full - 1) / (HEAD_PAIRS - full) * w.stages[1 - first]);
+		most += (w.tiles[1 - first] - fill + HEAD_PAIRS - 1) / HEAD_PAIRS * w.stages[1 - first];
+		time = (double)most * 0.27 + (n > 1 ? 3.0 + n * (double)tokens * (double)d * 8.0 / 6.5e6 : 0.0);
+		if (n == 1 || time < least * 0.98) {
+			least = time;
+			best = n;
 		}
 	}
 	return best;
@@ -1256,8 +1388,7 @@ head_plan plan_of(const anni_head_call *c, int grad)
 	p.row = take(&p.bytes, t * 4);
 	p.delta = take(&p.bytes, (int64_t)p.piece * t * 2 * p.terms);
 	p.ldd = (int)up(c->d_model, 8);
-	p.splits = split_dx(up(t, HEAD_TM) / HEAD_TM * (up(c->d_model, HEAD_TN) / HEAD_TN),
-	    up(std::min(p.piece, c->vocab), HEAD_TK) / HEAD_TK);
+	p.splits = c->dx ? split_dx(t, c->d_model, std::min(p.piece, c->vocab), p.terms, c->dw != NULL) : 1;
 	p.parts = c->dx && (p.splits > 1 || p.piece < c->vocab);
 	p.dxp = take(&p.bytes, p.parts ? p.splits * t * p.ldd * 4 : 0);
 	p.dbp = take(&p.bytes, c->dbias ? up(t, HEAD_HALF) / HEAD_HALF * c->vocab * 4 : 0);
@@ -1379,7 +1510,7 @@ int tensor_map(CUtensorMap *m, const void *base, int64_t cols, int64_t rows, int
 ** (devices beyond the table are asked every time).
 */
 #define HEAD_DEVICES	16
-std::atomic<int> known[4][HEAD_DEVICES];
+std::atomic<int> known[3][HEAD_DEVICES];
 std::atomic<int> known_rows[2][2][HEAD_DEVICES];
 
 template <typename K>
@@ -1404,45 +1535,56 @@ int ready(K kernel, int smem, int *sms, std::atomic<int> (*seen)[HEAD_DEVICES])
 	return ANNI_OK;
 }
 
-/* the product of one kind over the piece h.v0 .. h.v1 of the vocabulary */
+/* the products of one kind over the piece h.v0 .. h.v1 of the vocabulary */
 template <int KIND>
 int product(const head_args &h, cudaStream_t st)
 {
 	const int smem = HEAD_STAGES * HEAD_STAGE_BYTES + 1024;
 	const int width = h.v1 - h.v0;
+	const bool f32 = h.terms > 1;
 	gemm_args g;
 	int sms;
-	int rc;
+	int rc = ANNI_OK;
 
+	memset(&g, 0, sizeof(g));
 	g.h = h;
-	if (KIND == LOSS || KIND == DELTA) {
-		g.m_tiles = (int)tiles(h.tokens, HEAD_TM);
-		g.n_tiles = (int)tiles(width, HEAD_TN);
-		g.k_blocks = (int)tiles(h.d, HEAD_TK);
-		rc = tensor_map(&g.a, h.x, h.d, h.tokens, h.ldx, 1, HEAD_HALF);
-		rc = rc ? rc : tensor_map(&g.b, h.w, h.vocab, h.d, h.ldw, 1, HEAD_TK);
-	} else if (KIND == DX) {
-		g.m_tiles = (int)tiles(h.tokens, HEAD_TM);
-		g.n_tiles = (int)tiles(h.d, HEAD_TN);
-		g.k_blocks = (int)tiles(width, HEAD_TK);
-		rc = tensor_map(&g.a, h.delta, width, h.tokens, h.ldp, h.terms, HEAD_HALF);
-		rc = rc ? rc : tensor_map(&g.b, h.w, h.vocab, h.d, h.ldw, 1, HEAD_HALF);
+	if (KIND == GRAD) {
+		const grad_work w = work_of(h.tokens, h.d, width, h.terms, h.dx != NULL, h.dw != NULL, h.splits);
+		product_args &x = g.p[DX];
+		product_args &y = g.p[DW];
+
+		order(w, &g.first, &g.extra);
+		x.m_tiles = (int)tiles(h.tokens, HEAD_TM);
+		x.n_tiles = (int)tiles(h.d, HEAD_TN);
+		x.k_blocks = (int)tiles(width, HEAD_TK);
+		y.m_tiles = (int)tiles(h.d, HEAD_TM);
+		y.n_tiles = (int)tiles(width, HEAD_TN);
+		y.k_blocks = (int)tiles(h.tokens, HEAD_TK);
+		/* fp32 gradients are to be good to fp32; what is rounded to bf16 has no use for it */
+		x.run = f32 ? HEAD_RUN_F32 : x.k_blocks;
+		y.run = f32 ? HEAD_RUN_F32 : y.k_blocks;
+		x.total = (int)w.tiles[DX];
+		y.total = (int)w.tiles[DW];
+		rc = tensor_map(&x.a, h.delta, width, h.tokens, h.ldp, h.terms, HEAD_HALF);
+		rc = rc ? rc : tensor_map(&x.b, h.w, h.vocab, h.d, h.ldw, 1, HEAD_HALF);
+		rc = rc ? rc : tensor_map(&y.a, h.x, h.d, h.tokens, h.ldx, 1, HEAD_TK);
+		rc = rc ? rc : tensor_map(&y.b, h.delta, width, h.tokens, h.ldp, h.terms, HEAD_TK);
 	} else {
-		g.m_tiles = (int)tiles(h.d, HEAD_TM);
-		g.n_tiles = (int)tiles(width, HEAD_TN);
-		g.k_blocks = (int)tiles(h.tokens, HEAD_TK);
-		rc = tensor_map(&g.a, h.x, h.d, h.tokens, h.ldx, 1, HEAD_TK);
-		rc = rc ? rc : tensor_map(&g.b, h.delta, width, h.tokens, h.ldp, h.terms, HEAD_TK);
+		product_args &z = g.p[0];
+
+		z.m_tiles = (int)tiles(h.tokens, HEAD_TM);
+		z.n_tiles = (int)tiles(width, HEAD_TN);
+		z.k_blocks = (int)tiles(h.d, HEAD_TK);
+		z.run = KIND == LOSS || f32 ? HEAD_RUN : z.k_blocks;
+		z.total = z.m_tiles * z.n_tiles;
+		rc = tensor_map(&z.a, h.x, h.d, h.tokens, h.ldx, 1, HEAD_HALF);
+		rc = rc ? rc : tensor_map(&z.b, h.w, h.vocab, h.d, h.ldw, 1, HEAD_TK);
 	}
-	/* the losses and fp32 gradients are to be good to fp32; what is rounded to bf16 has no use for it */
-	g.run = KIND == LOSS || (KIND == DELTA && h.terms > 1) ? HEAD_RUN : h.terms > 1 ? HEAD_RUN_F32 : g.k_blocks;
+	rc = rc ? rc : ready(product_kernel<KIND>, smem, &sms, &known[KIND]);
 	if (rc != ANNI_OK)
 		return rc;
-	rc = ready(product_kernel<KIND>, smem, &sms, &known[KIND]);
-	if (rc != ANNI_OK)
-		return rc;
-	return launch(product_kernel<KIND>, 2 * std::min(sms / 2, g.m_tiles * g.n_tiles * (KIND == DX ? h.splits : 1)), HEAD_THREADS,
-	    smem, st, g);
+	return launch(product_kernel<KIND>, 2 * std::min<int64_t>(sms / 2, (int64_t)g.p[0].total + g.p[1].total), HEAD_THREADS, smem,
+	    st, g);
 }
 
 template <int ROWS>
@@ -1551,10 +1693,8 @@ extern "C" int anni_head_loss_grad(const anni_head_call *c, void *stream)
 	for (h.v0 = 0; rc == ANNI_OK && h.v0 < h.vocab; h.v0 = h.v1) {
 		h.v1 = std::min(h.vocab, h.v0 + p.piece);
 		rc = product<DELTA>(h, st);
-		if (rc == ANNI_OK && h.dx)
-			rc = product<DX>(h, st);
-		if (rc == ANNI_OK && h.dw)
-			rc = product<DW>(h, st);
+		if (rc == ANNI_OK && (h.dx || h.dw))
+			rc = product<GRAD>(h, st);
 	}
 	if (rc == ANNI_OK && h.dxp)
 		rc = launch(finish_dx_kernel, std::min(h.tokens, 16384), 128, 0, st, h);
