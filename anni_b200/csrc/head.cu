@@ -274,8 +274,9 @@ __device__ __forceinline__ void store32(void *p, const uint32_t (&r)[8])
 
 __device__ __forceinline__ void load32(const void *p, uint32_t (&r)[8])
 {
-	asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]),
-	    "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "l"(p) : "memory");
+	/* not volatile: nothing that a kernel loads this way has been stored by it before, so loads may go ahead of stores */
+	asm("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]),
+	    "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "l"(p));
 }
 
 __device__ __forceinline__ float to_f(__nv_bfloat16 v)
@@ -632,8 +633,8 @@ __device__ __forceinline__ void transpose(float (&v)[32])
 
 /*
 ** A warp's 32 x 32 results, lane l with row l, stored or added to what is there: at (row, col) of a matrix of which
-** `rows` rows and `left` of these columns exist.  Rows on 32 bytes: every lane whole sectors of its own row; others:
-** transposed, the warp row by row, so that its accesses are one piece whatever the address.
+** `rows` rows and `left` of these columns exist.  Rows on 32 bytes: every lane whole sectors of its own row; on 16 bytes: half
+** sectors; others: transposed, the warp row by row, so that its accesses are one piece whatever the address.
 */
 __device__ __forceinline__ void put_block(void *base, int64_t ld, int row, int rows, int64_t col, int left, float (&v)[32],
 	bool bf16, bool add)
@@ -676,6 +677,33 @@ __device__ __forceinline__ void put_block(void *base, int64_t ld, int row, int r
 		}
 		return;
 	}
+	if (left >= 32 && (((uintptr_t)base | (uintptr_t)(ld * size) | (uintptr_t)(col * size)) & 15) == 0) {
+		char *out = static_cast<char *>(base) + ((int64_t)(row + lane) * ld + col) * size;
+
+		if (row + lane >= rows)
+			return;
+#pragma unroll
+		for (int i = 0; i < 32; i += 4) {
+			if (bf16) {
+				uint2 r = add ? *reinterpret_cast<const uint2 *>(out + i * 2) : make_uint2(0, 0);
+				const float2 p = unpack2(r.x);
+				const float2 q = unpack2(r.y);
+
+				r.x = bf16_pair(p.x + v[i], p.y + v[i + 1]);
+				r.y = bf16_pair(q.x + v[i + 2], q.y + v[i + 3]);
+				*reinterpret_cast<uint2 *>(out + i * 2) = r;
+			} else {
+				float4 r = add ? *reinterpret_cast<const float4 *>(out + i * 4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+
+				r.x += v[i];
+				r.y += v[i + 1];
+				r.z += v[i + 2];
+				r.w += v[i + 3];
+				*reinterpret_cast<float4 *>(out + i * 4) = r;
+			}
+		}
+		return;
+	}
 	transpose(v);
 	if (lane >= left)
 		return;
@@ -714,6 +742,29 @@ __device__ __forceinline__ void put_block(void *base, int64_t ld, int row, int r
 			asm volatile("" ::: "memory");
 		}
 	}
+}
+
+/*
+** Results that are added to what is there: this thread's piece of its row on its way to the L2 while the products
+** run.  (Fetched from HBM when they are needed, piece by piece, they made an epilogue of 6,000 cycles one of 24,000.)
+*/
+__device__ __forceinline__ void fetch_ahead(const gemm_args &g, const tile_at &at)
+{
+	const head_args &h = g.h;
+	const bool dx = at.which == DX;
+	const int row = at.m0 + epi_row();
+	const int col = (dx ? 0 : h.v0) + at.n0 + epi_col();
+	const int size = !dx && h.bf16 ? 2 : 4;
+	const int left = min(128, (dx ? h.ldd : h.v1) - col);
+	const char *base = reinterpret_cast<const char *>(dx ? h.dxp + (int64_t)at.split * h.tokens * h.ldd : h.dw);
+
+	if (dx ? !h.dxp || h.v0 == 0 : !h.add)
+		return;
+	if (row >= (dx ? h.tokens : h.d))
+		return;
+	base += ((int64_t)row * (dx ? h.ldd : h.lddw) + col) * size;
+	for (int i = 0; i < left * size; i += 128)
+		asm volatile("prefetch.global.L2 [%0];" :: "l"(base + i));
 }
 
 __device__ __forceinline__ void grad_epilogue(const gemm_args &g, const tile_at &at, float (&acc)[4][32])
@@ -862,6 +913,8 @@ __device__ __forceinline__ void drainer(const gemm_args &g, gemm_smem *s, int ra
 			stage_bias(g.h, at.n0, g.h.vocab, s->epi.bias[b]);
 		if (KIND == DELTA)
 			stage_bias(g.h, g.h.v0 + at.n0, g.h.v1, s->epi.bias[b]);
+		if (KIND == GRAD)
+			fetch_ahead(g, at);
 #pragma unroll 1
 		for (int from = at.k0; from < at.k1; from += run, done++) {
 			const uint32_t addr = s->tmem + lanes + (done & 1) * HEAD_TN + epi_col();
@@ -1300,20 +1353,35 @@ size_t take(size_t *at, int64_t bytes)
 	return here;
 }
 
-/* tiles of the two products of the gradients over one piece of `width` columns, and stages of a tile (all terms) */
+/*
+** Tiles of the two products of the gradients over one piece of `width` columns, and how long a tile takes, in
+** stages of 512 cycles: its stages (all terms), but no less than its epilogue (`least`, for dw): 6,000 cycles, 14,000
+** where it adds to what is there, 20,000 where the rows of the result are off the 16-byte grid.
+*/
 struct grad_work {
 	int64_t	tiles[2];
 	int64_t	stages[2];
 };
 
-grad_work work_of(int64_t tokens, int64_t d, int64_t width, int terms, bool dx, bool dw, int splits)
+#define HEAD_EPI_STAGES		12
+#define HEAD_EPI_STAGES_ADD	28
+#define HEAD_EPI_STAGES_ODD	40
+
+/* an epilogue of dw, in stages */
+int epilogue_of_dw(const void *base, int64_t ld, bool bf16, bool add)
+{
+	return (((uintptr_t)base | (uintptr_t)(ld * (bf16 ? 2 : 4))) & 15) != 0 ? HEAD_EPI_STAGES_ODD
+	    : add ? HEAD_EPI_STAGES_ADD : HEAD_EPI_STAGES;
+}
+
+grad_work work_of(int64_t tokens, int64_t d, int64_t width, int terms, bool dx, bool dw, int splits, int least)
 {
 	grad_work w;
 
 	w.tiles[DX] = dx ? up(tokens, HEAD_TM) / HEAD_TM * (up(d, HEAD_TN) / HEAD_TN) * splits : 0;
 	w.tiles[DW] = dw ? up(d, HEAD_TM) / HEAD_TM * (up(width, HEAD_TN) / HEAD_TN) : 0;
-	w.stages[DX] = (up(width, HEAD_TK) / HEAD_TK * terms + splits - 1) / splits;
-	w.stages[DW] = up(tokens, HEAD_TK) / HEAD_TK * terms;
+	w.stages[DX] = std::max<int64_t>((up(width, HEAD_TK) / HEAD_TK * terms + splits - 1) / splits, HEAD_EPI_STAGES);
+	w.stages[DW] = std::max<int64_t>(up(tokens, HEAD_TK) / HEAD_TK * terms, least);
 	return w;
 }
 
@@ -1330,14 +1398,14 @@ void order(const grad_work &w, int *first, int *extra)
 ** With dw's tiles to fill the rounds one part is best for many rows; a few rows have few tiles of dx, whose sums
 ** are as long as the vocabulary (128 rows of 1536 against 100,000 entries: 6 tiles of 1563 stages).
 */
-int split_dx(int64_t tokens, int64_t d, int64_t width, int terms, bool dw)
+int split_dx(int64_t tokens, int64_t d, int64_t width, int terms, bool dw, int least_dw)
 {
 	const int64_t stages = up(width, HEAD_TK) / HEAD_TK;
 	int best = 1;
 	double least = 0.0;
 
 	for (int n = 1; n <= HEAD_PAIRS && (n == 1 || stages / n >= 4); n++) {
-		const grad_work w = work_of(tokens, d, width, terms, true, dw, n);
+		const grad_work w = work_of(tokens, d, width, terms, true, dw, n, least_dw);
 		int first;
 		int extra;
 		int64_t full;
@@ -1388,7 +1456,8 @@ head_plan plan_of(const anni_head_call *c, int grad)
 	p.row = take(&p.bytes, t * 4);
 	p.delta = take(&p.bytes, (int64_t)p.piece * t * 2 * p.terms);
 	p.ldd = (int)up(c->d_model, 8);
-	p.splits = c->dx ? split_dx(t, c->d_model, std::min(p.piece, c->vocab), p.terms, c->dw != NULL) : 1;
+	p.splits = c->dx ? split_dx(t, c->d_model, std::min(p.piece, c->vocab), p.terms, c->dw != NULL,
+	    epilogue_of_dw(c->dw, c->lddw, c->grad_dtype == ANNI_DT_BF16, (c->flags & ANNI_HEAD_ACCUMULATE) != 0)) : 1;
 	p.parts = c->dx && (p.splits > 1 || p.piece < c->vocab);
 	p.dxp = take(&p.bytes, p.parts ? p.splits * t * p.ldd * 4 : 0);
 	p.dbp = take(&p.bytes, c->dbias ? up(t, HEAD_HALF) / HEAD_HALF * c->vocab * 4 : 0);
@@ -1549,7 +1618,8 @@ int product(const head_args &h, cudaStream_t st)
 	memset(&g, 0, sizeof(g));
 	g.h = h;
 	if (KIND == GRAD) {
-		const grad_work w = work_of(h.tokens, h.d, width, h.terms, h.dx != NULL, h.dw != NULL, h.splits);
+		const grad_work w = work_of(h.tokens, h.d, width, h.terms, h.dx != NULL, h.dw != NULL, h.splits,
+		    epilogue_of_dw(h.dw, h.lddw, h.bf16, h.add));
 		product_args &x = g.p[DX];
 		product_args &y = g.p[DW];
 
