@@ -15,13 +15,15 @@
 **
 ** Rows: a target below 0 is ignored (nll 0, no gradient; x[t] may hold anything), a target >= vocab
 ** gives nll NaN and no gradient, and a row whose factor grad_scale * weight[t] is 0 has no gradient
-** either, whatever x[t] holds.  A bias of -inf masks an entry of the vocabulary; a row with nothing left
-** has nll NaN and no gradient.
+** either, whatever x[t] holds.  A bias of -inf masks an entry of the vocabulary (its column of W must still be
+** finite); a row with nothing left has nll NaN and no gradient.
 **
 ** Arithmetic: products of bf16 values in fp32 accumulators; maximum, sum, exponentials in fp32.  For
 ** bf16 gradients delta is rounded once to bf16 as the operand of the two products; for fp32 gradients
 ** it is carried as three bf16 terms (24 bits), so dx and dw are good to fp32.  dbias is summed in fp32
-** from the unrounded delta.  Sums run in a fixed order: the same inputs give the same bits.
+** from the unrounded delta.  The tensor cores cut sums off instead of rounding them; the logits of the loss, and with
+** fp32 gradients every sum, are therefore taken in runs of 512 or 256 terms that are added up rounded.  Sums
+** run in a fixed order: the same inputs give the same bits.
 **
 ** Waits inside the kernels are bounded: a block that gives up (two seconds without progress) fills what it
 ** has not computed with NaN, which shows in nll, dx, dw and dbias.

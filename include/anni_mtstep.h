@@ -29,7 +29,7 @@
 ** Calls on one handle belong on one stream, one after another (a step changes its tensors in place
 ** anyway); different handles are independent.  Every call works on the device the handle was created
 ** on, whichever device is current.  Steps and anni_mtstep_set_grads can be captured into a graph: the
-** values of hp and seed are then those of the capture, and a replayed step takes the gradient addresses that the
+** handle then has to live as long as the graph; the values of hp and seed are those of the capture, and a replayed step takes the gradient addresses that the
 ** last anni_mtstep_set_grads before it, replayed or not, has left.
 */
 #ifndef ANNI_MTSTEP_H__
