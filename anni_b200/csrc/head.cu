@@ -8,7 +8,9 @@
 **           (three terms of it for fp32 gradients), and its column sums for dbias
 **   grad    dx = delta W^T of the piece, added to an fp32 sum over the pieces, and dw = x^T delta of the piece, stored
 **           or added to the gradient; together, so that the tiles of one fill the rounds that the other leaves open
-** Bound by the tensor cores: 2 T D V operations each (the logits twice, since they are not kept).
+** Bound by the tensor cores: 2 T D V operations each (the logits twice, since they are not kept).  4096 rows of 1536
+** against 100,000 entries: loss 867 us (1.45 PFLOP/s, 0.86 of the rate of a library product), delta 966, dx and dw 1.7 ms
+** one by one; back to back at the power limit 4.2 ms in all, where four library products would take 3.6 ms.
 **
 ** Two blocks (a cluster on two neighbouring SMs) work on a 256 x 256 tile: each keeps 128 rows of the result
 ** and loads its 128 rows of the one operand and 128 of the other by TMA into a ring of HEAD_STAGES stages; one
@@ -258,6 +260,25 @@ __device__ __forceinline__ float exp2_approx(float x)
 	return r;
 }
 
+/* two floats in one instruction: a += b, a = a b + c, a *= b */
+__device__ __forceinline__ void add2(float &a0, float &a1, float b0, float b1)
+{
+	asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tadd.rn.f32x2 x, x, y;\n\t"
+	    "mov.b64 {%0, %1}, x;\n\t}" : "+f"(a0), "+f"(a1) : "f"(b0), "f"(b1));
+}
+
+__device__ __forceinline__ void fma2(float &a0, float &a1, float b, float c)
+{
+	asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %2};\n\tmov.b64 z, {%3, %3};\n\t"
+	    "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}" : "+f"(a0), "+f"(a1) : "f"(b), "f"(c));
+}
+
+__device__ __forceinline__ void mul2(float &a0, float &a1, float b)
+{
+	asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %2};\n\tmul.rn.f32x2 x, x, y;\n\t"
+	    "mov.b64 {%0, %1}, x;\n\t}" : "+f"(a0), "+f"(a1) : "f"(b));
+}
+
 __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi)
 {
 	const __nv_bfloat162 q = __floats2bfloat162_rn(lo, hi);
@@ -465,6 +486,7 @@ __device__ __forceinline__ void loss_epilogue(const gemm_args &g, const tile_at 
 	const int rel = y >= at.n0 + c0 && y < h.vocab && y < at.n0 + c0 + 128 ? y - at.n0 - c0 : -1;
 	float top = -INFINITY;
 	float sum = 0.0f;
+	float sum1 = 0.0f;
 
 #pragma unroll
 	for (int c = 0; c < 4; c++) {
@@ -476,10 +498,8 @@ __device__ __forceinline__ void loss_epilogue(const gemm_args &g, const tile_at 
 		for (int i = 0; i < 32; i += 4) {
 			const float4 b = *reinterpret_cast<const float4 *>(bias + c0 + c * 32 + i);
 
-			v[i] += b.x;
-			v[i + 1] += b.y;
-			v[i + 2] += b.z;
-			v[i + 3] += b.w;
+			add2(v[i], v[i + 1], b.x, b.y);
+			add2(v[i + 2], v[i + 3], b.z, b.w);
 		}
 		if (__any_sync(0xffffffffu, rel >= c * 32 && rel < c * 32 + 32)) {	/* one in vocab / 32 chunks of a row */
 #pragma unroll
@@ -493,12 +513,22 @@ __device__ __forceinline__ void loss_epilogue(const gemm_args &g, const tile_at 
 			high = fmaxf(high, v[i]);	/* a NaN shows in the sum */
 		high = fmaxf(high, top);
 		base = high == -INFINITY ? 0.0f : high;
-		sum *= exp2_approx((top - base) * LOG2E);
+		mul2(sum, sum1, exp2_approx((top - base) * LOG2E));
 		top = high;
+		if (__any_sync(0xffffffffu, fabsf(base) > 1e30f)) {	/* a mask of lowest values: the product would overflow */
 #pragma unroll
-		for (int i = 0; i < 32; i++)
-			sum += exp2_approx((v[i] - base) * LOG2E);
+			for (int i = 0; i < 32; i++)
+				sum += exp2_approx((v[i] - base) * LOG2E);
+			continue;
+		}
+		base *= -LOG2E;
+#pragma unroll
+		for (int i = 0; i < 32; i += 2) {
+			fma2(v[i], v[i + 1], LOG2E, base);
+			add2(sum, sum1, exp2_approx(v[i]), exp2_approx(v[i + 1]));
+		}
 	}
+	sum += sum1;
 	if (c0)
 		half[epi_row()] = make_float2(top, sum);
 	epi_barrier();
@@ -520,7 +550,7 @@ __device__ __forceinline__ void delta_epilogue(const gemm_args &g, const tile_at
 	const int c0 = epi_col();
 	const int t = at.m0 + epi_row();
 	const float f = t < h.tokens ? h.row[t] : 0.0f;
-	const float lse = f != 0.0f ? h.lse[t] : 0.0f;
+	const float lse = f != 0.0f ? -h.lse[t] : -INFINITY;	/* negated; no gradient: all exponentials 0 */
 	const int y = f != 0.0f ? h.target[t] - h.v0 - at.n0 - c0 : -1;
 	__nv_bfloat16 *out = h.delta + (int64_t)t * h.ldp + at.n0 + c0;
 
@@ -532,10 +562,15 @@ __device__ __forceinline__ void delta_epilogue(const gemm_args &g, const tile_at
 		for (int i = 0; i < 32; i += 4) {
 			const float4 b = *reinterpret_cast<const float4 *>(bias + c0 + c * 32 + i);
 
-			v[i] = exp2_approx((v[i] + b.x - lse) * LOG2E);
-			v[i + 1] = exp2_approx((v[i + 1] + b.y - lse) * LOG2E);
-			v[i + 2] = exp2_approx((v[i + 2] + b.z - lse) * LOG2E);
-			v[i + 3] = exp2_approx((v[i + 3] + b.w - lse) * LOG2E);
+			add2(v[i], v[i + 1], b.x, b.y);
+			add2(v[i + 2], v[i + 3], b.z, b.w);
+		}
+#pragma unroll
+		for (int i = 0; i < 32; i += 2) {
+			add2(v[i], v[i + 1], lse, lse);
+			mul2(v[i], v[i + 1], LOG2E);
+			v[i] = exp2_approx(v[i]);
+			v[i + 1] = exp2_approx(v[i + 1]);
 		}
 		if (__any_sync(0xffffffffu, y >= c * 32 && y < c * 32 + 32)) {
 #pragma unroll
@@ -544,8 +579,8 @@ __device__ __forceinline__ void delta_epilogue(const gemm_args &g, const tile_at
 					v[i] -= 1.0f;
 		}
 #pragma unroll
-		for (int i = 0; i < 32; i++)
-			v[i] = f != 0.0f ? v[i] * f : 0.0f;
+		for (int i = 0; i < 32; i += 2)
+			mul2(v[i], v[i + 1], f);
 		if (t < h.tokens) {
 			__nv_bfloat16 *q = out + c * 32;
 
@@ -1036,10 +1071,10 @@ __device__ __forceinline__ void join(float &top, float &sum, float2 p)
 
 /*
 ** The loss of one row or two: W is read once and little is computed, so HBM is the bound, and a product whose
-** tiles have 256 rows spends longer on the empty ones (1536 x 100,000: one row 93 us there and 65 us here, two rows
-** 91 and 64, four rows 92 and 119; reading W alone takes 47 us).  A block takes 256 entries of the vocabulary, each
-** of its eight warps an eighth of the rows of W: ROWS x 8 sums a thread, in fp32, added up over the warps in
-** order.  VEC: lane l has columns 8 l .. 8 l + 7, else (no 16-byte grid) columns l, l + 32, ...
+** tiles have 256 rows spends longer on the empty ones (1536 x 100,000: one row 93 us there and 68 us here, two rows
+** 91 and 74, four rows 92 and 119; reading W alone takes 47 us).  A block takes 256 entries of the vocabulary, each
+** of its eight warps an eighth of the rows of W (sixteen warps: 73 us): ROWS x 8 sums a thread, in fp32, added
+** up over the warps in order.  VEC: lane l has columns 8 l .. 8 l + 7, else (no 16-byte grid) columns l, l + 32, ...
 */
 template <int ROWS, bool VEC>
 __global__ void __launch_bounds__(256) rows_kernel(const head_args h)

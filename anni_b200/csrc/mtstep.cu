@@ -4,8 +4,10 @@
 ** Every tensor is cut into whole tiles of ANNI_MT_TILE elements, which a table lists with their tensors, and
 ** what is left of it, which a second table lists: two loops, the first without a thought for ends.  A block
 ** takes a tile at a time, each of its eight warps a run of ANNI_MT_BLOCK = 256 elements -- the run that
-** shares a scale in the 8-bit form, so that the two block maxima are reductions inside a warp.  The step is bound by HBM: 28 bytes per element with 32-bit
-** moments, bf16 gradients and twins, 16 with 8-bit moments.
+** shares a scale in the 8-bit form, so that the two block maxima are reductions inside a warp.  The step is
+** bound by HBM: 28 bytes per element with 32-bit moments, bf16 gradients and twins, 16 with 8-bit moments.
+** 184.7 M elements, with the norm: 0.95 ms (0.83 of the copy rate for those bytes) and 0.60 ms (0.75); 98.5 M,
+** fp32 gradients, stochastic, no norm: 0.32 ms (0.76).
 */
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>

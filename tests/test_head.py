@@ -251,6 +251,13 @@ def test_large_logits_and_lowest_bias():
     for a in (dx, dw, db):
         assert torch.isfinite(a).all()
     assert not dw[:, 100:300].any()
+    b.fill_(torch.finfo(torch.float32).min)         # nothing but the lowest value: an even softmax, for one row and for many
+    for rows in (1, 40):
+        nll, lse = head_loss(x[:rows], w, target[:rows], bias=b)
+        assert torch.isfinite(lse).all() and (lse < -3e38).all()
+        dbias = torch.empty(v, device="cuda")
+        head_loss_grad(x[:rows], w, target[:rows], lse, bias=b, dbias=dbias)
+        assert torch.isfinite(dbias).all()
 
 
 @gpu

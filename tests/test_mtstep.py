@@ -424,6 +424,19 @@ def test_the_same_inputs_give_the_same_bits():
 
 
 @gpu
+@pytest.mark.parametrize("state_dtype", [DT_F32, DT_Q8])
+def test_nothing_to_step(state_dtype):
+    """Empty tensors alone, and tensors that all sit out: the step closes, the norm is 0."""
+    for n in (0, 5000):
+        p = torch.ones(n, device="cuda")
+        s = MultiStep([p, torch.zeros(0, device="cuda")], grads=[torch.zeros(0, device="cuda") if n == 0 else None, None],
+                      state_dtype=state_dtype)
+        s.step(hyper(1.0))
+        st = s.status()
+        assert st.error == 0 and st.skipped == 0 and st.norm == 0.0 and st.steps_done == 1 and (p == 1).all()
+
+
+@gpu
 def test_python_refusals():
     p, g = torch.zeros(8, device="cuda"), torch.zeros(8, device="cuda")
     for bad in (dict(grads=[g[:4]]), dict(grads=[g, g]), dict(decay=[True, False]), dict(twins=[g]),
