@@ -89,6 +89,7 @@ class MultiStep:
                 raise TypeError(f"MultiStep: gradients are all float32 or all bfloat16, got {sorted(map(str, kinds))}")
             grad_dtype = _GRAD_DT[kinds.pop()] if kinds else DT_F32
         self.params, self.grad_dtype, self.state_dtype = params, grad_dtype, state_dtype
+        self.counts = [p.numel() for p in params]
         self.device = params[0].device
         if self.device.type != "cuda":
             raise RuntimeError("anni_b200 needs a CUDA device: there is no CPU path")
@@ -109,19 +110,22 @@ class MultiStep:
         self._check("m", self.m, torch.float8_e4m3fn if eight else torch.float32)
         self._check("v", self.v, torch.float8_e5m2 if eight else torch.float32)
         if eight:
-            self._check("m_scale", self.m_scale, torch.float32, _blocks)
-            self._check("v_scale", self.v_scale, torch.float32, _blocks)
+            blocks = [_blocks(k) for k in self.counts]
+            self._check("m_scale", self.m_scale, torch.float32, blocks)
+            self._check("v_scale", self.v_scale, torch.float32, blocks)
         self._check("twins", self.twins, torch.bfloat16, none=True)
         self._check_grads(grads)
         if len(decay) != n:
             raise ValueError("MultiStep: decay needs one entry per parameter")
         arr = (Tensor * n)()
-        at = lambda xs, k: xs[k].data_ptr() if xs is not None and xs[k] is not None and xs[k].numel() else None  # noqa: E731
-        for k in range(n):
-            arr[k].param, arr[k].grad, arr[k].m, arr[k].v = (at(x, k) for x in (params, grads, self.m, self.v))
-            arr[k].m_scale, arr[k].v_scale, arr[k].twin_bf16 = (at(x, k) for x in (self.m_scale, self.v_scale, self.twins))
-            arr[k].n = params[k].numel()
-            arr[k].flags = (SEG_WD if decay[k] else 0) | (SEG_TWIN_BF16 if self.twins[k] is not None else 0)
+        # of entries without elements the library looks at nothing but the count
+        for field, xs in (("param", params), ("grad", grads), ("m", self.m), ("v", self.v), ("m_scale", self.m_scale),
+                          ("v_scale", self.v_scale), ("twin_bf16", self.twins)):
+            for t, x in zip(arr, xs or ()):
+                if x is not None and x.numel():
+                    setattr(t, field, x.data_ptr())
+        for t, k, wd, twin in zip(arr, self.counts, decay, self.twins):
+            t.n, t.flags = k, (SEG_WD if wd else 0) | (SEG_TWIN_BF16 if twin is not None else 0)
         self.grads = grads
         self.L = lib()
         h = C.c_void_p()
@@ -129,16 +133,17 @@ class MultiStep:
             check("anni_mtstep_create", self.L.anni_mtstep_create(arr, n, grad_dtype, state_dtype, C.byref(h)))
         self.h = h
 
-    def _check(self, what, xs, dtype, count=lambda n: n, none=False):
+    def _check(self, what, xs, dtype, counts=None, none=False):
         if len(xs) != len(self.params):
             raise ValueError(f"MultiStep: {what} needs one entry per parameter")
-        for k, x in enumerate(xs):
+        dev = self.device.index
+        for k, (x, n) in enumerate(zip(xs, self.counts if counts is None else counts)):
             if none and x is None:
                 continue
-            if x.dtype != dtype or x.device != self.device or not x.is_contiguous():
+            if x.dtype is not dtype or x.get_device() != dev or not x.is_contiguous():
                 raise TypeError(f"MultiStep: {what}[{k}] must be a contiguous {dtype} tensor on {self.device}")
-            if x.numel() != count(self.params[k].numel()):
-                raise ValueError(f"MultiStep: {what}[{k}] has {x.numel()} elements, not {count(self.params[k].numel())}")
+            if x.numel() != n:
+                raise ValueError(f"MultiStep: {what}[{k}] has {x.numel()} elements, not {n}")
 
     def _check_grads(self, grads):
         self._check("grads", grads, torch.bfloat16 if self.grad_dtype == DT_BF16 else torch.float32, none=True)
