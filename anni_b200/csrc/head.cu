@@ -54,6 +54,9 @@
 #define HEAD_PIECE_BYTES ((size_t)256 << 20)	/* of delta in the workspace */
 #define HEAD_TERMS	3	/* bf16 terms of delta for fp32 gradients */
 #define HEAD_FEW_DIM	8192	/* rows_kernel keeps two rows of x in shared memory */
+#define ROWS_ODD_TN	(HEAD_TN - 8)	/* its tile where the rows of W are off the 16-byte grid */
+#define ROWS_DEEP	64	/* rows of W that a block has at least, */
+#define ROWS_START	512	/* and those that a round of blocks takes in time to start and end */
 #define HEAD_WAIT_NS	2000000000ull	/* a wait inside a kernel gives up after this long */
 
 namespace {
@@ -133,6 +136,14 @@ __device__ __forceinline__ uint32_t smem_in(uint32_t addr, uint32_t rank)
 
 	asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
 	return r;
+}
+
+__device__ __forceinline__ float load_in(uint32_t cluster_addr)
+{
+	float v;
+
+	asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+	return v;
 }
 
 __device__ __forceinline__ void mbar_arrive_in(uint32_t cluster_bar)
@@ -1071,48 +1082,59 @@ __device__ __forceinline__ void join(float &top, float &sum, float2 p)
 
 /*
 ** The loss of one row or two: W is read once and little is computed, so HBM is the bound, and a product whose
-** tiles have 256 rows spends longer on the empty ones (1536 x 100,000: one row 93 us there and 68 us here, two rows
-** 91 and 74, four rows 92 and 119; reading W alone takes 47 us).  A block takes 256 entries of the vocabulary, each
-** of its eight warps an eighth of the rows of W (sixteen warps: 73 us): ROWS x 8 sums a thread, in fp32, added
-** up over the warps in order.  VEC: lane l has columns 8 l .. 8 l + 7, else (no 16-byte grid) columns l, l + 32, ...
+** tiles have 256 rows spends longer on the empty ones (one row, 1536 x 100,000: 58 us here, 89 there, and reading W
+** alone takes 47; 1536 x 4097, off the 16-byte grid: 10 and 21; 2560 x 32,768: 32 and 53).
+** A block takes `width` entries of the vocabulary and `deep` rows of W, each of its eight warps every eighth of these:
+** ROWS x 8 sums a thread, in fp32, added up over the warps and then over the blocks of a cluster, which
+** share the rows of the same entries, in order.
+** Loads are of 16-byte granules.  In rows off that grid a warp's granules all begin the same number of entries ahead of
+** the tile, since eight rows on an address is the same modulo 16 bytes: its sums just belong to entries that many
+** places to the left, and a tile has eight entries less.  What such granules hold of other rows goes into
+** sums that nobody reads; those that reach out of W are read one entry at a time.
 */
-template <int ROWS, bool VEC>
-__global__ void __launch_bounds__(256) rows_kernel(const head_args h)
+template <int ROWS>
+__global__ void __launch_bounds__(256) rows_kernel(const head_args h, int width, int deep, int parts)
 {
-	extern __shared__ float xs[];		/* [d][ROWS] */
+	extern __shared__ float xs[];		/* [deep][ROWS] */
 	__shared__ float red[8][HEAD_TN];
+	__shared__ float sums[ROWS][HEAD_TN];
 	__shared__ float2 warps[8];
 	const int lane = threadIdx.x & 31;
 	const int w = threadIdx.x >> 5;
-	const int v0 = blockIdx.x * HEAD_TN;
-	const int lo = (int)((int64_t)h.d * w / 8);
-	const int hi = (int)((int64_t)h.d * (w + 1) / 8);
+	const int tile = blockIdx.x / parts;
+	const int rank = blockIdx.x % parts;	/* in the cluster */
+	const int v0 = tile * width;
+	const int lo = min(rank * deep, h.d);
+	const int hi = min(lo + deep, h.d);
+	const int shift = (int)((uintptr_t)(h.w + (int64_t)(lo + w) * h.ldw) & 15) / 2;
+	const int c0 = v0 - shift + lane * 8;	/* this thread's entries */
+	const int64_t total = (int64_t)(h.d - 1) * h.ldw + h.vocab;
 	const int mine = v0 + threadIdx.x;
 	float acc[ROWS][8];
 
 	dependent();
-	for (int i = threadIdx.x; i < h.d * ROWS; i += 256)
-		xs[i] = to_f(h.x[(int64_t)(i % ROWS) * h.ldx + i / ROWS]);
+	for (int i = threadIdx.x; i < (hi - lo) * ROWS; i += 256)
+		xs[i] = to_f(h.x[(int64_t)(i % ROWS) * h.ldx + lo + i / ROWS]);
 #pragma unroll
 	for (int r = 0; r < ROWS; r++)
 #pragma unroll
 		for (int j = 0; j < 8; j++)
 			acc[r][j] = 0.0f;
 	__syncthreads();
-	for (int d0 = lo; d0 < hi; d0 += 8) {
+	for (int d0 = lo + w; d0 < hi; d0 += 64) {
 		uint32_t q[8][4];
 
 #pragma unroll
 		for (int k = 0; k < 8; k++) {
-			const __nv_bfloat16 *row = h.w + (int64_t)(d0 + k) * h.ldw + v0;
+			const int64_t e = (int64_t)(d0 + k * 8) * h.ldw + c0;
 
 #pragma unroll
 			for (int j = 0; j < 4; j++)
 				q[k][j] = 0;
-			if (d0 + k >= hi)
+			if (d0 + k * 8 >= hi || c0 >= h.vocab)
 				continue;
-			if (VEC && v0 + lane * 8 + 8 <= h.vocab) {
-				const uint4 r = __ldcs(reinterpret_cast<const uint4 *>(row + lane * 8));
+			if (e >= 0 && e + 8 <= total) {
+				const uint4 r = __ldcs(reinterpret_cast<const uint4 *>(h.w + e));
 
 				q[k][0] = r.x;
 				q[k][1] = r.y;
@@ -1120,16 +1142,13 @@ __global__ void __launch_bounds__(256) rows_kernel(const head_args h)
 				q[k][3] = r.w;
 			} else
 #pragma unroll
-				for (int j = 0; j < 8; j++) {
-					const int c = VEC ? lane * 8 + j : lane + 32 * j;
-
-					if (v0 + c < h.vocab)
-						q[k][j / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(row)[c] << (j % 2 * 16);
-				}
+				for (int j = 0; j < 8; j++)
+					if (c0 + j >= 0 && c0 + j < h.vocab)
+						q[k][j / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(h.w)[e + j] << (j % 2 * 16);
 		}
 #pragma unroll
 		for (int k = 0; k < 8; k++) {
-			if (d0 + k >= hi)
+			if (d0 + k * 8 >= hi)
 				break;
 #pragma unroll
 			for (int j = 0; j < 8; j += 2) {
@@ -1137,7 +1156,7 @@ __global__ void __launch_bounds__(256) rows_kernel(const head_args h)
 
 #pragma unroll
 				for (int r = 0; r < ROWS; r++) {
-					const float a = xs[(d0 + k) * ROWS + r];
+					const float a = xs[(d0 + k * 8 - lo) * ROWS + r];
 
 					acc[r][j] = fmaf(a, b.x, acc[r][j]);
 					acc[r][j + 1] = fmaf(a, b.y, acc[r][j + 1]);
@@ -1148,23 +1167,45 @@ __global__ void __launch_bounds__(256) rows_kernel(const head_args h)
 #pragma unroll
 	for (int r = 0; r < ROWS; r++) {
 		float z = 0.0f;
-		float top;
-		float sum;
 
 		__syncthreads();
 #pragma unroll
 		for (int j = 0; j < 8; j++)
-			red[w][VEC ? lane * 8 + j : lane + 32 * j] = acc[r][j];
+			if (lane * 8 + j >= shift)
+				red[w][lane * 8 + j - shift] = acc[r][j];
 		__syncthreads();
+		if ((int)threadIdx.x < width)
 #pragma unroll
-		for (int k = 0; k < 8; k++)
-			z += red[k][threadIdx.x];
-		if (mine >= h.vocab)
-			z = -INFINITY;
-		else if (h.bias)
-			z += h.bias[mine];
-		if (mine < h.vocab && h.target[r] == mine)
-			h.hit[r] = z;
+			for (int k = 0; k < 8; k++)
+				z += red[k][threadIdx.x];
+		sums[r][threadIdx.x] = z;
+	}
+	if (parts > 1) {
+		cluster_barrier();
+		if (rank == 0)
+#pragma unroll
+			for (int r = 0; r < ROWS; r++) {
+				float z = sums[r][threadIdx.x];
+
+				for (int k = 1; k < parts; k++)
+					z += load_in(smem_in(smem_of(&sums[r][threadIdx.x]), k));
+				sums[r][threadIdx.x] = z;
+			}
+		cluster_barrier();	/* nobody leaves before its sums have been read */
+		if (rank != 0)
+			return;
+	}
+#pragma unroll
+	for (int r = 0; r < ROWS; r++) {
+		float z = -INFINITY;
+		float top;
+		float sum;
+
+		if ((int)threadIdx.x < width && mine < h.vocab) {
+			z = sums[r][threadIdx.x] + (h.bias ? h.bias[mine] : 0.0f);
+			if (h.target[r] == mine)
+				h.hit[r] = z;
+		}
 		top = z;
 #pragma unroll
 		for (int k = 16; k > 0; k >>= 1)
@@ -1173,13 +1214,14 @@ __global__ void __launch_bounds__(256) rows_kernel(const head_args h)
 #pragma unroll
 		for (int k = 16; k > 0; k >>= 1)
 			sum += __shfl_xor_sync(0xffffffffu, sum, k);
+		__syncthreads();
 		if (lane == 0)
 			warps[w] = make_float2(top, sum);
 		__syncthreads();
 		if (threadIdx.x == 0) {
 			for (int k = 1; k < 8; k++)
 				join(top, sum, warps[k]);
-			h.part[(int64_t)blockIdx.x * h.tokens + r] = make_float2(top, sum);
+			h.part[(int64_t)tile * h.tokens + r] = make_float2(top, sum);
 		}
 	}
 }
@@ -1481,7 +1523,7 @@ head_plan plan_of(const anni_head_call *c, int grad)
 	p.w = take(&p.bytes, p.copy_w ? c->d_model * p.ldw * 2 : 0);
 	if (!grad) {
 		p.hit = take(&p.bytes, t * 4);
-		p.part = take(&p.bytes, up(c->vocab, HEAD_TN) / HEAD_TN * t * 8);
+		p.part = take(&p.bytes, up(c->vocab, ROWS_ODD_TN) / ROWS_ODD_TN * t * 8);
 		return p;
 	}
 	p.terms = c->grad_dtype == ANNI_DT_BF16 ? 1 : HEAD_TERMS;
@@ -1548,25 +1590,35 @@ unsigned tiles(int64_t n, int64_t of)
 ** up meanwhile and wait (dependent()) before they touch memory.
 */
 template <typename... P, typename... A>
-int launch(void (*kernel)(P...), int64_t grid, int threads, int smem, cudaStream_t st, A... args)
+int launch_clusters(void (*kernel)(P...), int64_t grid, int threads, int smem, cudaStream_t st, int cluster, A... args)
 {
 	cudaLaunchConfig_t cfg = {};
-	cudaLaunchAttribute early;
+	cudaLaunchAttribute attrs[2];
 
-	early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-	early.val.programmaticStreamSerializationAllowed = 1;
+	attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+	attrs[0].val.programmaticStreamSerializationAllowed = 1;
+	attrs[1].id = cudaLaunchAttributeClusterDimension;
+	attrs[1].val.clusterDim.x = (unsigned)cluster;
+	attrs[1].val.clusterDim.y = 1;
+	attrs[1].val.clusterDim.z = 1;
 	cfg.gridDim = dim3((unsigned)grid);
 	cfg.blockDim = dim3((unsigned)threads);
 	cfg.dynamicSmemBytes = (size_t)smem;
 	cfg.stream = st;
-	cfg.attrs = &early;
-	cfg.numAttrs = 1;
+	cfg.attrs = attrs;
+	cfg.numAttrs = cluster > 1 ? 2 : 1;	/* 1: none, or the kernel's own */
 	if (cudaLaunchKernelEx(&cfg, kernel, P(args)...) != cudaSuccess) {
 		(void)cudaGetLastError();
 		return ANNI_E_CUDA;
 	}
 	anni_count_launch();
 	return ANNI_OK;
+}
+
+template <typename... P, typename... A>
+int launch(void (*kernel)(P...), int64_t grid, int threads, int smem, cudaStream_t st, A... args)
+{
+	return launch_clusters(kernel, grid, threads, smem, st, 1, args...);
 }
 
 /* blocks of 256 threads with 16 bytes each */
@@ -1615,7 +1667,7 @@ int tensor_map(CUtensorMap *m, const void *base, int64_t cols, int64_t rows, int
 */
 #define HEAD_DEVICES	16
 std::atomic<int> known[3][HEAD_DEVICES];
-std::atomic<int> known_rows[2][2][HEAD_DEVICES];
+std::atomic<int> known_rows[2][HEAD_DEVICES];
 
 template <typename K>
 int ready(K kernel, int smem, int *sms, std::atomic<int> (*seen)[HEAD_DEVICES])
@@ -1693,17 +1745,31 @@ int product(const head_args &h, cudaStream_t st)
 }
 
 template <int ROWS>
-int loss_rows(const head_args &h, bool vec, cudaStream_t st)
+int loss_rows(const head_args &h, int width, cudaStream_t st)
 {
-	const int smem = h.d * ROWS * 4;
+	const int n = (int)tiles(h.vocab, width);
+	int64_t least = 0;
+	int parts = 1;
+	int deep;
 	int sms;
-	int rc = vec ? ready(rows_kernel<ROWS, true>, ROWS * HEAD_FEW_DIM * 4, &sms, &known_rows[ROWS - 1][1])
-	    : ready(rows_kernel<ROWS, false>, ROWS * HEAD_FEW_DIM * 4, &sms, &known_rows[ROWS - 1][0]);
+	int rc = ready(rows_kernel<ROWS>, ROWS * HEAD_FEW_DIM * 4, &sms, &known_rows[ROWS - 1]);
 
-	if (rc != ANNI_OK)
-		return rc;
-	return vec ? launch(rows_kernel<ROWS, true>, tiles(h.vocab, HEAD_TN), 256, smem, st, h)
-	    : launch(rows_kernel<ROWS, false>, tiles(h.vocab, HEAD_TN), 256, smem, st, h);
+	/*
+	** Few entries: the rows of W are split, so that every SM has blocks that read (1536 x 300, 8 us, unsplit 44).  Blocks
+	** that run at a time: four an SM with one row (61 registers), three with two (68); a round that few blocks
+	** are left for costs as much as a full one (two rows, 1536 x 65,536: 59 us in 512 blocks, 51 in 256).
+	*/
+	for (int p = 1; p <= 8 && (p == 1 || h.d >= p * ROWS_DEEP); p++) {
+		const int64_t rounds = ((int64_t)n * p + (5 - ROWS) * 2 * HEAD_PAIRS - 1) / ((5 - ROWS) * 2 * HEAD_PAIRS);
+		const int64_t time = rounds * (h.d / p + ROWS_START);
+
+		if (p == 1 || time < least) {
+			least = time;
+			parts = p;
+		}
+	}
+	deep = (int)up((h.d + parts - 1) / parts, 8);	/* a warp's rows are then eight apart from block to block, too */
+	return rc ? rc : launch_clusters(rows_kernel<ROWS>, (int64_t)n * parts, 256, deep * ROWS * 4, st, parts, h, width, deep, parts);
 }
 
 /* the copies that the plan asks for; x's with the factors of the rows when gradients follow */
@@ -1743,6 +1809,7 @@ extern "C" int anni_head_loss(const anni_head_call *c, void *stream)
 	int rc = check(c, 0);
 	head_plan p;
 	head_args h;
+	int width = HEAD_TN;
 
 	if (rc != ANNI_OK || c->tokens == 0)
 		return rc;
@@ -1754,13 +1821,12 @@ extern "C" int anni_head_loss(const anni_head_call *c, void *stream)
 	rc = pack(c, p, h, false, st);
 	h.v1 = h.vocab;
 	if (rc == ANNI_OK && p.few) {
-		const bool vec = (h.ldw & 7) == 0 && ((uintptr_t)h.w & 15) == 0;
-
-		rc = h.tokens == 1 ? loss_rows<1>(h, vec, st) : loss_rows<2>(h, vec, st);
+		width = (h.ldw & 7) || ((uintptr_t)h.w & 15) ? ROWS_ODD_TN : HEAD_TN;
+		rc = h.tokens == 1 ? loss_rows<1>(h, width, st) : loss_rows<2>(h, width, st);
 	} else if (rc == ANNI_OK)
 		rc = product<LOSS>(h, st);
 	if (rc == ANNI_OK)
-		rc = launch(join_kernel, tiles(h.tokens, 32), 1024, 0, st, h, (int)tiles(h.vocab, HEAD_TN));
+		rc = launch(join_kernel, tiles(h.tokens, 32), 1024, 0, st, h, (int)tiles(h.vocab, width));
 	return rc;
 }
 

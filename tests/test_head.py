@@ -451,3 +451,22 @@ def test_every_declared_symbol_is_exported():
     from test_abi_cpu import _declared_symbols
     names = _declared_symbols("anni_head.h")
     assert len(names) == 4 and not [k for k in names if not hasattr(head.lib(), k)]
+
+
+@gpu
+@pytest.mark.parametrize("t", [1, 2, 3])
+@pytest.mark.parametrize("d,v,ld,at", [(1536, 4097, 4097, 0), (2567, 1001, 1001, 0), (700, 20001, 20001, 0), (1, 9, 9, 0),
+                                       (9, 7, 7, 0), (513, 496, 500, 3), (130, 260, 264, 1), (200, 1000, 1008, 8),
+                                       (8192, 300, 302, 0), (64, 248, 249, 1), (1200, 33000, 33000, 0)])
+def test_few_rows_of_any_layout(t, d, v, ld, at):
+    """A few rows read W in whole 16-byte granules wherever its rows begin; what lies between them is NaN."""
+    x, w, target, b = inputs(t, d, v, seed=t + d + v)
+    target[0] = v - 1
+    wide = torch.full((d * ld + at,), float("nan"), dtype=BF, device="cuda")
+    view = wide[at:at + (d - 1) * ld + v].as_strided((d, v), (ld, 1))
+    view.copy_(w)
+    ex = Exact(x, w, target, b)
+    first = head_loss(x, view, target, bias=b)
+    check_loss(ex, *first)
+    for again in zip(first, head_loss(x, view, target, bias=b)):
+        assert torch.equal(*again)
