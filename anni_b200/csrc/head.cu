@@ -835,6 +835,23 @@ __device__ __forceinline__ void grad_epilogue(const gemm_args &g, const tile_at 
 		}
 }
 
+/* dbias of the columns from, from + step, ... below `to`: delta's column sums of all rows of tiles, in order */
+__device__ __forceinline__ void finish_db(const head_args &h, int from, int to, int step)
+{
+	const int tiles = (h.tokens + HEAD_HALF - 1) / HEAD_HALF;
+
+	for (int v = from; v < to; v += step) {
+		double s = 0.0;
+
+#pragma unroll 8
+		for (int k = 0; k < tiles; k++)
+			s += (double)h.dbp[(int64_t)k * h.vocab + v];
+		if (h.add)
+			s += h.bf16 ? (double)to_f(static_cast<__nv_bfloat16 *>(h.db)[v]) : (double)static_cast<float *>(h.db)[v];
+		put(h.db, v, (float)s, h.bf16, 0);
+	}
+}
+
 /* ---- the product -------------------------------------------------------------------------------------- */
 
 struct gemm_smem {
@@ -1057,6 +1074,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HEAD_THREADS, 1) pro
 			producer<KIND>(g, &s, ring, rank, pair, pairs);
 		if (warp == 1 && (threadIdx.x & 31) == 0 && rank == 0)
 			multiplier<KIND>(g, &s, ring, pair, pairs);
+		/* nothing waits for dbias: a warp that is idle otherwise, beside the products */
+		if (KIND == GRAD && warp == 3 && g.h.db)
+			finish_db(g.h, g.h.v0 + blockIdx.x * 32 + (threadIdx.x & 31), g.h.v1, gridDim.x * 32);
 	} else
 		drainer<KIND>(g, &s, rank, pair, pairs);
 	__syncwarp();
@@ -1270,37 +1290,49 @@ __device__ __forceinline__ float row_factor(const head_args &h, int t)
 	return y >= 0 && y < h.vocab && h.lse[t] != -INFINITY ? h.scale * (h.weight ? h.weight[t] : 1.0f) : 0.0f;
 }
 
+/* a matrix to be copied to rows on the 16-byte grid, by so many blocks */
+struct pack_job {
+	__nv_bfloat16		*to;
+	const __nv_bfloat16	*from;
+	int64_t			ldf;
+	int			ldt;
+	int			rows;
+	int			cols;
+	int			blocks;
+};
+
 /*
-** Rows of bf16 to a 16-byte grid, 16 bytes a thread.  With ROWS also their factors, and zeros for the rows
+** The copies of x and w, 16 bytes a thread.  With `factors` also those of x's rows, and zeros for the rows
 ** without a gradient, so that whatever they hold meets a delta of 0 as 0.
 */
-template <bool ROWS>
-__global__ void __launch_bounds__(256) pack_kernel(const head_args h, __nv_bfloat16 *to, int ldt, const __nv_bfloat16 *from,
-	int64_t ldf, int rows, int cols)
+__global__ void __launch_bounds__(256) pack_kernel(const head_args h, const pack_job x, const pack_job w, int factors)
 {
-	const int per = ldt / 8;
-	const int64_t total = (int64_t)rows * per;
+	const bool is_x = (int)blockIdx.x < x.blocks;
+	const pack_job &p = is_x ? x : w;
+	const int block = is_x ? blockIdx.x : blockIdx.x - x.blocks;
+	const int per = p.ldt / 8;
+	const int64_t total = (int64_t)p.rows * per;
 
 	dependent();
-	for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+	for (int64_t i = (int64_t)block * 256 + threadIdx.x; i < total; i += (int64_t)p.blocks * 256) {
 		const int r = (int)(i / per);
 		const int c = (int)(i - (int64_t)r * per) * 8;
-		const float f = ROWS ? row_factor(h, r) : 1.0f;
-		const __nv_bfloat16 *src = from + (int64_t)r * ldf + c;
+		const float f = is_x && factors ? row_factor(h, r) : 1.0f;
+		const __nv_bfloat16 *src = p.from + (int64_t)r * p.ldf + c;
 		uint32_t q[4] = { 0, 0, 0, 0 };
 
-		if (ROWS && c == 0)
+		if (is_x && factors && c == 0)
 			h.row[r] = f;
 		if (f != 0.0f) {
-			if (c + 8 <= cols && ((uintptr_t)src & 15) == 0)
+			if (c + 8 <= p.cols && ((uintptr_t)src & 15) == 0)
 				*reinterpret_cast<uint4 *>(q) = *reinterpret_cast<const uint4 *>(src);
 			else
 #pragma unroll
 				for (int j = 0; j < 8; j++)
-					if (c + j < cols)
+					if (c + j < p.cols)
 						q[j / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(src)[j] << (j % 2 * 16);
 		}
-		*reinterpret_cast<uint4 *>(to + (int64_t)r * ldt + c) = make_uint4(q[0], q[1], q[2], q[3]);
+		*reinterpret_cast<uint4 *>(p.to + (int64_t)r * p.ldt + c) = make_uint4(q[0], q[1], q[2], q[3]);
 	}
 }
 
@@ -1340,19 +1372,11 @@ __global__ void __launch_bounds__(128) finish_dx_kernel(const head_args h)
 	}
 }
 
-__global__ void __launch_bounds__(256) finish_db_kernel(const head_args h, int tiles)
+/* where no product of gradients follows, which would do it */
+__global__ void __launch_bounds__(256) finish_db_kernel(const head_args h)
 {
-	const int v = blockIdx.x * blockDim.x + threadIdx.x;
-	double s = 0.0;
-
 	dependent();
-	if (v >= h.vocab)
-		return;
-	for (int k = 0; k < tiles; k++)
-		s += (double)h.dbp[(int64_t)k * h.vocab + v];
-	if (h.add)
-		s += h.bf16 ? (double)to_f(static_cast<__nv_bfloat16 *>(h.db)[v]) : (double)static_cast<float *>(h.db)[v];
-	put(h.db, v, (float)s, h.bf16, 0);
+	finish_db(h, blockIdx.x * blockDim.x + threadIdx.x, h.vocab, gridDim.x * blockDim.x);
 }
 
 /* ---- host --------------------------------------------------------------------------------------- */
@@ -1772,23 +1796,15 @@ int loss_rows(const head_args &h, int width, cudaStream_t st)
 	return rc ? rc : launch_clusters(rows_kernel<ROWS>, (int64_t)n * parts, 256, deep * ROWS * 4, st, parts, h, width, deep, parts);
 }
 
-/* the copies that the plan asks for; x's with the factors of the rows when gradients follow */
+/* the copies that the plan asks for, in one launch; x's with the factors of the rows when gradients follow */
 int pack(const anni_head_call *c, const head_plan &p, const head_args &h, bool grad, cudaStream_t st)
 {
-	__nv_bfloat16 *x = const_cast<__nv_bfloat16 *>(h.x);
-	__nv_bfloat16 *w = const_cast<__nv_bfloat16 *>(h.w);
-	int rc = ANNI_OK;
+	const pack_job x = { const_cast<__nv_bfloat16 *>(h.x), static_cast<const __nv_bfloat16 *>(c->x), c->ldx, (int)p.ldx, h.tokens,
+	    h.d, p.copy_x ? (int)blocks(h.tokens, p.ldx) : 0 };
+	const pack_job w = { const_cast<__nv_bfloat16 *>(h.w), static_cast<const __nv_bfloat16 *>(c->w), c->ldw, (int)p.ldw, h.d,
+	    h.vocab, p.copy_w ? (int)blocks(h.d, p.ldw) : 0 };
 
-	if (grad)
-		rc = launch(pack_kernel<true>, blocks(h.tokens, h.ldx), 256, 0, st, h, x, (int)h.ldx,
-		    static_cast<const __nv_bfloat16 *>(c->x), c->ldx, h.tokens, h.d);
-	else if (p.copy_x)
-		rc = launch(pack_kernel<false>, blocks(h.tokens, h.ldx), 256, 0, st, h, x, (int)h.ldx,
-		    static_cast<const __nv_bfloat16 *>(c->x), c->ldx, h.tokens, h.d);
-	if (rc == ANNI_OK && p.copy_w)
-		rc = launch(pack_kernel<false>, blocks(h.d, h.ldw), 256, 0, st, h, w, (int)h.ldw,
-		    static_cast<const __nv_bfloat16 *>(c->w), c->ldw, h.d, h.vocab);
-	return rc;
+	return x.blocks + w.blocks == 0 ? ANNI_OK : launch(pack_kernel, x.blocks + w.blocks, 256, 0, st, h, x, w, (int)grad);
 }
 
 }	/* namespace */
@@ -1869,7 +1885,7 @@ extern "C" int anni_head_loss_grad(const anni_head_call *c, void *stream)
 	}
 	if (rc == ANNI_OK && h.dxp)
 		rc = launch(finish_dx_kernel, std::min(h.tokens, 16384), 128, 0, st, h);
-	if (rc == ANNI_OK && h.db)
-		rc = launch(finish_db_kernel, tiles(h.vocab, 256), 256, 0, st, h, (int)tiles(h.tokens, HEAD_HALF));
+	if (rc == ANNI_OK && h.db && !h.dx && !h.dw)
+		rc = launch(finish_db_kernel, tiles(h.vocab, 256), 256, 0, st, h);
 	return rc;
 }
