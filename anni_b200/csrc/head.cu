@@ -271,17 +271,11 @@ __device__ __forceinline__ float exp2_approx(float x)
 	return r;
 }
 
-/* two floats in one instruction: a += b, a = a b + c, a *= b */
+/* two floats in one instruction: a += b, a *= b */
 __device__ __forceinline__ void add2(float &a0, float &a1, float b0, float b1)
 {
 	asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tadd.rn.f32x2 x, x, y;\n\t"
 	    "mov.b64 {%0, %1}, x;\n\t}" : "+f"(a0), "+f"(a1) : "f"(b0), "f"(b1));
-}
-
-__device__ __forceinline__ void fma2(float &a0, float &a1, float b, float c)
-{
-	asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %2};\n\tmov.b64 z, {%3, %3};\n\t"
-	    "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}" : "+f"(a0), "+f"(a1) : "f"(b), "f"(c));
 }
 
 __device__ __forceinline__ void mul2(float &a0, float &a1, float b)
@@ -526,16 +520,10 @@ __device__ __forceinline__ void loss_epilogue(const gemm_args &g, const tile_at 
 		base = high == -INFINITY ? 0.0f : high;
 		mul2(sum, sum1, exp2_approx((top - base) * LOG2E));
 		top = high;
-		if (__any_sync(0xffffffffu, fabsf(base) > 1e30f)) {	/* a mask of lowest values: the product would overflow */
 #pragma unroll
-			for (int i = 0; i < 32; i++)
-				sum += exp2_approx((v[i] - base) * LOG2E);
-			continue;
-		}
-		base *= -LOG2E;
-#pragma unroll
-		for (int i = 0; i < 32; i += 2) {
-			fma2(v[i], v[i + 1], LOG2E, base);
+		for (int i = 0; i < 32; i += 2) {	/* the difference first: a rounded product of a mask's size is anything */
+			add2(v[i], v[i + 1], -base, -base);
+			mul2(v[i], v[i + 1], LOG2E);
 			add2(sum, sum1, exp2_approx(v[i]), exp2_approx(v[i + 1]));
 		}
 	}

@@ -15,8 +15,9 @@
 **
 ** Rows: a target below 0 is ignored (nll 0, no gradient; x[t] may hold anything), a target >= vocab
 ** gives nll NaN and no gradient, and a row whose factor grad_scale * weight[t] is 0 has no gradient
-** either, whatever x[t] holds.  A bias of -inf masks an entry of the vocabulary (its column of W must still be
-** finite); a row with nothing left has nll NaN and no gradient.
+** either, whatever x[t] holds.  A bias of -inf, or a finite one far below the other logits, masks an entry of
+** the vocabulary (its column of W must still be finite); a row with nothing but -inf left has nll NaN and no
+** gradient.
 **
 ** Arithmetic: products of bf16 values in fp32 accumulators; maximum, sum, exponentials in fp32.  For
 ** bf16 gradients delta is rounded once to bf16 as the operand of the two products; for fp32 gradients
