@@ -35,12 +35,9 @@
 #include <atomic>
 #include <mutex>
 #include "anni_head.h"
+#include "head_plan.h"
 #include "optstep_internal.h"
 
-#define HEAD_TM		256	/* rows and columns of a tile */
-#define HEAD_TN		256
-#define HEAD_HALF	128	/* rows of the result, and of either operand, in each block of the pair */
-#define HEAD_TK		64	/* 128 bytes of bf16: the widest swizzle */
 #define HEAD_STAGES	6
 #define HEAD_A_BYTES	(HEAD_HALF * HEAD_TK * 2)
 #define HEAD_B_BYTES	(HEAD_HALF * HEAD_TK * 2)
@@ -50,11 +47,6 @@
 #define HEAD_THREADS	(128 + HEAD_EPI)
 #define HEAD_RUN	8	/* stages in one run of a sum: 512 terms of a logit, */
 #define HEAD_RUN_F32	4	/* 256 of an fp32 gradient */
-#define HEAD_PAIRS	74	/* pairs of SMs that the work is cut for; any number of them runs it */
-#define HEAD_PIECE_BYTES ((size_t)256 << 20)	/* of delta in the workspace */
-#define HEAD_TERMS	3	/* bf16 terms of delta for fp32 gradients */
-#define HEAD_FEW_DIM	8192	/* rows_kernel keeps two rows of x in shared memory */
-#define ROWS_ODD_TN	(HEAD_TN - 8)	/* its tile where the rows of W are off the 16-byte grid */
 #define ROWS_DEEP	64	/* rows of W that a block has at least, */
 #define ROWS_START	512	/* and those that a round of blocks takes in time to start and end */
 #define HEAD_WAIT_NS	2000000000ull	/* a wait inside a kernel gives up after this long */
@@ -62,7 +54,6 @@
 namespace {
 
 enum { LOSS, DELTA, GRAD };
-enum { DX, DW };	/* the products of GRAD */
 
 struct head_args {
 	const __nv_bfloat16	*x;
@@ -379,8 +370,8 @@ __device__ __forceinline__ bool tile_of(const gemm_args &g, int i, int rank, int
 		n = t % p.n_tiles;
 		m = t / p.n_tiles % p.m_tiles;
 		r.split = t / (p.n_tiles * p.m_tiles);
-		r.k0 = (int)((int64_t)p.k_blocks * r.split / g.h.splits);
-		r.k1 = (int)((int64_t)p.k_blocks * (r.split + 1) / g.h.splits);
+		r.k0 = part_begin(p.k_blocks, r.split, g.h.splits);
+		r.k1 = part_begin(p.k_blocks, r.split + 1, g.h.splits);
 	} else if (KIND == GRAD) {
 		m = t % p.m_tiles;
 		n = t / p.m_tiles;
@@ -1369,40 +1360,6 @@ __global__ void __launch_bounds__(256) finish_db_kernel(const head_args h)
 
 /* ---- host --------------------------------------------------------------------------------------- */
 
-int64_t up(int64_t n, int64_t to)
-{
-	return (n + to - 1) / to * to;
-}
-
-/* the loss by rows_kernel, which takes x and w as they are */
-bool few_rows(const anni_head_call *c)
-{
-	return c->tokens <= 2 && c->d_model <= HEAD_FEW_DIM;
-}
-
-/* where things lie in the workspace (byte offsets), and how the work is cut */
-struct head_plan {
-	size_t	x;		/* copies of x and w on a 16-byte grid, where needed */
-	size_t	w;
-	int	few;		/* rows_kernel */
-	int	copy_x;
-	int	copy_w;
-	int64_t	ldx;
-	int64_t	ldw;
-	size_t	hit;
-	size_t	part;
-	size_t	row;
-	size_t	delta;
-	size_t	dxp;
-	size_t	dbp;
-	size_t	bytes;
-	int	piece;
-	int	terms;
-	int	splits;
-	int	parts;		/* dx is added up in fp32 in the workspace */
-	int	ldd;
-};
-
 int check(const anni_head_call *c, int grad)
 {
 	if (!c || c->tokens < 0 || c->d_model < 1 || c->vocab < 1)
@@ -1432,125 +1389,6 @@ int check_buffers(const anni_head_call *c, int grad, size_t need)
 	if (((uintptr_t)c->bias | (uintptr_t)c->target | (uintptr_t)c->lse | (uintptr_t)c->nll | (uintptr_t)c->weight) & 3)
 		return ANNI_E_ARG;
 	return ((uintptr_t)c->workspace & 255) || c->workspace_bytes < need ? ANNI_E_ARG : ANNI_OK;
-}
-
-size_t take(size_t *at, int64_t bytes)
-{
-	const size_t here = *at;
-
-	*at = (size_t)up((int64_t)here + bytes, 256);
-	return here;
-}
-
-/*
-** Tiles of the two products of the gradients over one piece of `width` columns, and how long a tile takes, in
-** stages of 512 cycles: its stages (all terms), but no less than its epilogue (`least`, for dw): 6,000 cycles, 14,000
-** where it adds to what is there, 20,000 where the rows of the result are off the 16-byte grid.
-*/
-struct grad_work {
-	int64_t	tiles[2];
-	int64_t	stages[2];
-};
-
-#define HEAD_EPI_STAGES		12
-#define HEAD_EPI_STAGES_ADD	28
-#define HEAD_EPI_STAGES_ODD	40
-
-/* an epilogue of dw, in stages */
-int epilogue_of_dw(const void *base, int64_t ld, bool bf16, bool add)
-{
-	return (((uintptr_t)base | (uintptr_t)(ld * (bf16 ? 2 : 4))) & 15) != 0 ? HEAD_EPI_STAGES_ODD
-	    : add ? HEAD_EPI_STAGES_ADD : HEAD_EPI_STAGES;
-}
-
-grad_work work_of(int64_t tokens, int64_t d, int64_t width, int terms, bool dx, bool dw, int splits, int least)
-{
-	grad_work w;
-
-	w.tiles[DX] = dx ? up(tokens, HEAD_TM) / HEAD_TM * (up(d, HEAD_TN) / HEAD_TN) * splits : 0;
-	w.tiles[DW] = dw ? up(d, HEAD_TM) / HEAD_TM * (up(width, HEAD_TN) / HEAD_TN) : 0;
-	w.stages[DX] = std::max<int64_t>((up(width, HEAD_TK) / HEAD_TK * terms + splits - 1) / splits, HEAD_EPI_STAGES);
-	w.stages[DW] = std::max<int64_t>(up(tokens, HEAD_TK) / HEAD_TK * terms, least);
-	return w;
-}
-
-/* which product goes first, and how many tiles of the other make up for one of it */
-void order(const grad_work &w, int *first, int *extra)
-{
-	*first = w.stages[DX] >= w.stages[DW] ? DX : DW;
-	*extra = (int)((w.stages[*first] + w.stages[1 - *first] / 2) / w.stages[1 - *first]);
-}
-
-/*
-** Into how many parts the sum over the vocabulary in dx is cut: as many as make the busiest pair of SMs finish
-** first.  A stage takes a pair 512 cycles (0.27 us); every part is written and read once more as fp32, at 6.5 TB/s.
-** With dw's tiles to fill the rounds one part is best for many rows; a few rows have few tiles of dx, whose sums
-** are as long as the vocabulary (128 rows of 1536 against 100,000 entries: 6 tiles of 1563 stages).
-*/
-int split_dx(int64_t tokens, int64_t d, int64_t width, int terms, bool dw, int least_dw)
-{
-	const int64_t stages = up(width, HEAD_TK) / HEAD_TK;
-	int best = 1;
-	double least = 0.0;
-
-	for (int n = 1; n <= HEAD_PAIRS && (n == 1 || stages / n >= 4); n++) {
-		const grad_work w = work_of(tokens, d, width, terms, true, dw, n, least_dw);
-		int first;
-		int extra;
-		int64_t full;
-		int64_t fill;
-		int64_t most;
-		int64_t least_long;
-		double time;
-
-		order(w, &first, &extra);
-		full = w.tiles[first] % HEAD_PAIRS;
-		least_long = w.tiles[first] / HEAD_PAIRS * w.stages[first];
-		fill = std::min(w.tiles[1 - first], (HEAD_PAIRS - full) * extra);
-		/* pairs with one more of the long tiles, and those that got short ones for it; then the rest for all */
-		most = std::max(full ? least_long + w.stages[first] : 0,
-		    least_long + (fill + HEAD_PAIRS - full - 1) / (HEAD_PAIRS - full) * w.stages[1 - first]);
-		most += (w.tiles[1 - first] - fill + HEAD_PAIRS - 1) / HEAD_PAIRS * w.stages[1 - first];
-		time = (double)most * 0.27 + (n > 1 ? 3.0 + n * (double)tokens * (double)d * 8.0 / 6.5e6 : 0.0);
-		if (n == 1 || time < least * 0.98) {
-			least = time;
-			best = n;
-		}
-	}
-	return best;
-}
-
-head_plan plan_of(const anni_head_call *c, int grad)
-{
-	head_plan p;
-	const int64_t t = std::max<int64_t>(c->tokens, 1);
-
-	memset(&p, 0, sizeof(p));
-	p.few = !grad && few_rows(c);
-	p.copy_x = grad || (!p.few && ((c->ldx & 7) || ((uintptr_t)c->x & 15)));
-	p.copy_w = !p.few && ((c->ldw & 7) || ((uintptr_t)c->w & 15));
-	p.ldx = up(c->d_model, 8);
-	p.ldw = up(c->vocab, 8);
-	p.x = take(&p.bytes, p.copy_x ? t * p.ldx * 2 : 0);
-	p.w = take(&p.bytes, p.copy_w ? c->d_model * p.ldw * 2 : 0);
-	if (!grad) {
-		p.hit = take(&p.bytes, t * 4);
-		p.part = take(&p.bytes, up(c->vocab, ROWS_ODD_TN) / ROWS_ODD_TN * t * 8);
-		return p;
-	}
-	p.terms = c->grad_dtype == ANNI_DT_BF16 ? 1 : HEAD_TERMS;
-	/* as many columns of delta as HEAD_PIECE_BYTES hold, then pieces of about the same size */
-	p.piece = (int)std::max<int64_t>(HEAD_TN, (int64_t)(HEAD_PIECE_BYTES / (size_t)(t * 2 * p.terms)) / HEAD_TN * HEAD_TN);
-	p.piece = (int)up((c->vocab + (c->vocab + p.piece - 1) / p.piece - 1) / ((c->vocab + p.piece - 1) / p.piece), HEAD_TN);
-	p.row = take(&p.bytes, t * 4);
-	p.delta = take(&p.bytes, (int64_t)p.piece * t * 2 * p.terms);
-	p.ldd = (int)up(c->d_model, 8);
-	p.splits = c->dx ? split_dx(t, c->d_model, std::min(p.piece, c->vocab), p.terms, c->dw != NULL,
-	    epilogue_of_dw(c->dw, c->lddw, c->grad_dtype == ANNI_DT_BF16, (c->flags & ANNI_HEAD_ACCUMULATE) != 0)) : 1;
-	p.parts = c->dx && (p.splits > 1 || p.piece < c->vocab);
-	p.dxp = take(&p.bytes, p.parts ? p.splits * t * p.ldd * 4 : 0);
-	p.dbp = take(&p.bytes, c->dbias ? up(t, HEAD_HALF) / HEAD_HALF * c->vocab * 4 : 0);
-	return p;
 }
 
 head_args args_of(const anni_head_call *c, const head_plan &p)
@@ -1717,7 +1555,8 @@ int product(const head_args &h, cudaStream_t st)
 	memset(&g, 0, sizeof(g));
 	g.h = h;
 	if (KIND == GRAD) {
-		const grad_work w = work_of(h.tokens, h.d, width, h.terms, h.dx != NULL, h.dw != NULL, h.splits,
+		const int splits = g.h.splits = parts_of(h.splits, width);
+		const grad_work w = work_of(h.tokens, h.d, width, h.terms, h.dx != NULL, h.dw != NULL, splits,
 		    epilogue_of_dw(h.dw, h.lddw, h.bf16, h.add));
 		product_args &x = g.p[DX];
 		product_args &y = g.p[DW];
