@@ -1,7 +1,9 @@
 """Loss of a language model's head and its gradients (``include/anni_head.h``).
 
 ``head_loss`` and ``head_loss_grad`` take torch tensors, allocate their workspace from torch for the length of
-the call and run on the current stream; nothing is kept between calls.
+the call and run on the current stream; nothing is kept between calls.  With ``stream=`` they run there: the caller
+orders the two streams, and all tensors of the call stay allocated until that stream has finished with them.  The
+results carry no autograd history: the gradients are ``head_loss_grad``'s.
 """
 import contextlib
 import ctypes as C
@@ -85,6 +87,14 @@ def _here(device, stream):
     return both
 
 
+def _used_on(stream, *tensors):
+    """The memory of these tensors is not handed out again before `stream` has done what is queued on it when they die."""
+    if stream is not None:
+        for t in tensors:
+            if t is not None:
+                t.record_stream(stream)
+
+
 def _run(name, c, grad, device):
     L = lib()
     need = C.c_size_t()
@@ -99,10 +109,13 @@ def head_loss(x, w, target, *, bias=None, stream=None):
     """Rows of (nll, lse): x bf16 (tokens, d_model), w bf16 (d_model, vocab), target int32 (tokens), bias fp32
     (vocab) or None.  A target below 0 is ignored (nll 0), one beyond the vocabulary gives NaN."""
     c = _call(x, w, target, bias)
+    caller = None if stream is None else torch.cuda.current_stream(x.device)
     with _here(x.device, stream):
         nll, lse = torch.empty(2, c.tokens, dtype=torch.float32, device=x.device).unbind(0)
         c.nll, c.lse = nll.data_ptr(), lse.data_ptr()
         _run("anni_head_loss", c, 0, x.device)
+    _used_on(stream, x, w, target, bias)
+    _used_on(caller, nll)               # lse is of the same storage; both were allocated on `stream`
     return nll, lse
 
 
@@ -128,3 +141,4 @@ def head_loss_grad(x, w, target, lse, *, bias=None, weight=None, grad_scale=1.0,
         c.dbias = _flat("dbias", dbias, c.vocab, kind, x.device)
     with _here(x.device, stream):
         _run("anni_head_loss_grad", c, 1, x.device)
+    _used_on(stream, x, w, target, lse, bias, weight, dx, dw, dbias)
