@@ -72,7 +72,9 @@ class MultiStep:
     float8_e4m3fn, ``v`` float8_e5m2, ``m_scale`` and ``v_scale`` fp32 per 256 elements); zeroed state is
     made here unless ``moments=(m, v)`` and, for DT_Q8, ``scales=(m_scale, v_scale)`` hand it in.
 
-    Calls on one object belong on one stream.  Every call works on the list's device.
+    Calls on one object belong on one stream.  Every call works on the list's device.  Gradients given to a call with
+    ``stream=`` stay allocated until that stream has finished with them, also when others have replaced them; those
+    that a captured step reads are the caller's to keep for as long as it is replayed.
     """
 
     def __init__(self, params, *, grads=None, state_dtype=DT_F32, grad_dtype=None, decay=None, twins=None,
@@ -126,7 +128,7 @@ class MultiStep:
                     setattr(t, field, x.data_ptr())
         for t, k, wd, twin in zip(arr, self.counts, decay, self.twins):
             t.n, t.flags = k, (SEG_WD if wd else 0) | (SEG_TWIN_BF16 if twin is not None else 0)
-        self.grads = grads
+        self.grads, self.grads_on = grads, None
         self.L = lib()
         h = C.c_void_p()
         with torch.cuda.device(self.device):
@@ -152,19 +154,29 @@ class MultiStep:
         s = torch.cuda.current_stream(self.device) if stream is None else stream
         return C.c_void_p(s.cuda_stream)
 
+    def _hold_grads(self, stream):
+        """The gradients' memory is not handed out again before `stream` has done what is queued on it when they go."""
+        if stream is not None and self.grads_on != stream.cuda_stream:
+            for g in self.grads:
+                if g is not None:
+                    g.record_stream(stream)
+            self.grads_on = stream.cuda_stream
+
     def set_grads(self, grads, stream=None):
         """New gradient tensors (None: sits out) for the steps queued after this call on the same stream."""
         grads = list(grads)
         self._check_grads(grads)
         arr = (C.c_void_p * len(grads))(*[g.data_ptr() if g is not None and g.numel() else None for g in grads])
         check("anni_mtstep_set_grads", self.L.anni_mtstep_set_grads(self.h, arr, self._stream(stream)))
-        self.grads = grads
+        self.grads, self.grads_on = grads, None
+        self._hold_grads(stream)
 
     def step(self, hp, *, seed=0, grads=None, stream=None):
         """One step (``hp`` from ``OptStep.hyper``); ``seed`` chooses the random bits of STEP_STOCHASTIC."""
         if grads is not None:
             self.set_grads(grads, stream)
         check("anni_mtstep_step", self.L.anni_mtstep_step(self.h, C.byref(hp), seed & (2 ** 64 - 1), self._stream(stream)))
+        self._hold_grads(stream)
 
     def status(self, stream=None):
         st = capi.Status()

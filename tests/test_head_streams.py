@@ -10,7 +10,7 @@ from anni_b200.head import head_loss, head_loss_grad
 from test_head import BF, inputs
 
 gpu = pytest.mark.gpu
-CYCLES = 20_000_000             # about 10 ms of a stream kept busy
+CYCLES = 200_000_000            # about 100 ms of a stream kept busy
 T, D, V = 2048, 512, 4096       # blocks of megabytes, which the allocator hands out whole
 
 
