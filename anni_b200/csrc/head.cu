@@ -22,8 +22,10 @@
 **
 ** The tensor cores cut their running sums off instead of rounding them: over K terms a result drifts towards zero
 ** by about 3e-9 K of its size (measured: log-sum-exp of 1001 terms low by 3.6e-6, an fp32 gradient over 8192
-** rows off by 2.5e-5).  Where that matters a sum is taken in runs: the warps that empty an accumulator add it to sums in
-** their registers, rounded, and the next run starts from zero.
+** rows off by 2.5e-5; terms of one sign: up to 7e-9 K, 5.6 % of a sum over 8.4 M rows).  A sum is therefore taken in
+** runs: the warps that empty an accumulator add it to sums in their registers, rounded, and the next run starts from
+** zero.  A run has 512 terms for the loss, 256 for fp32 gradients, and for bf16 gradients, whose rounding is 2^-8, as
+** many as cost nothing that could be measured: 16,384, and 4096 of a logit (4096 x 1536 x 100,000: 4.07 ms, in one run 4.08).
 */
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -46,7 +48,9 @@
 #define HEAD_EPI	256	/* threads that empty accumulators: 128 rows x 2 halves of the columns */
 #define HEAD_THREADS	(128 + HEAD_EPI)
 #define HEAD_RUN	8	/* stages in one run of a sum: 512 terms of a logit, */
-#define HEAD_RUN_F32	4	/* 256 of an fp32 gradient */
+#define HEAD_RUN_F32	4	/* 256 of an fp32 gradient, */
+#define HEAD_RUN_BF16	256	/* 16,384 of one that is rounded to bf16, */
+#define HEAD_RUN_DELTA	64	/* 4096 of a logit whose exponential is rounded to bf16 */
 #define ROWS_DEEP	64	/* rows of W that a block has at least, */
 #define ROWS_START	512	/* and those that a round of blocks takes in time to start and end */
 #define HEAD_WAIT_NS	2000000000ull	/* a wait inside a kernel gives up after this long */
@@ -1568,9 +1572,8 @@ int product(const head_args &h, cudaStream_t st)
 		y.m_tiles = (int)tiles(h.d, HEAD_TM);
 		y.n_tiles = (int)tiles(width, HEAD_TN);
 		y.k_blocks = (int)tiles(h.tokens, HEAD_TK);
-		/* fp32 gradients are to be good to fp32; what is rounded to bf16 has no use for it */
-		x.run = f32 ? HEAD_RUN_F32 : x.k_blocks;
-		y.run = f32 ? HEAD_RUN_F32 : y.k_blocks;
+		/* fp32 gradients are to be good to fp32; 1.1e-4 of a sum is a thirty-fifth of half a step of bf16 */
+		x.run = y.run = f32 ? HEAD_RUN_F32 : HEAD_RUN_BF16;
 		x.total = (int)w.tiles[DX];
 		y.total = (int)w.tiles[DW];
 		rc = tensor_map(&x.a, h.delta, width, h.tokens, h.ldp, h.terms, HEAD_HALF);
@@ -1583,7 +1586,8 @@ int product(const head_args &h, cudaStream_t st)
 		z.m_tiles = (int)tiles(h.tokens, HEAD_TM);
 		z.n_tiles = (int)tiles(width, HEAD_TN);
 		z.k_blocks = (int)tiles(h.d, HEAD_TK);
-		z.run = KIND == LOSS || f32 ? HEAD_RUN : z.k_blocks;
+		/* a logit's error is a relative one of delta: of a logit of 20 a seventh of half a step of bf16 */
+		z.run = KIND == LOSS || f32 ? HEAD_RUN : HEAD_RUN_DELTA;
 		z.total = z.m_tiles * z.n_tiles;
 		rc = tensor_map(&z.a, h.x, h.d, h.tokens, h.ldx, 1, HEAD_HALF);
 		rc = rc ? rc : tensor_map(&z.b, h.w, h.vocab, h.d, h.ldw, 1, HEAD_TK);

@@ -22,9 +22,10 @@
 ** Arithmetic: products of bf16 values in fp32 accumulators; maximum, sum, exponentials in fp32.  For
 ** bf16 gradients delta is rounded once to bf16 as the operand of the two products; for fp32 gradients
 ** it is carried as three bf16 terms (24 bits), so dx and dw are good to fp32.  dbias is summed in fp32
-** from the unrounded delta.  The tensor cores cut sums off instead of rounding them; the logits of the loss, and with
-** fp32 gradients every sum, are therefore taken in runs of 512 or 256 terms that are added up rounded.  Sums
-** run in a fixed order: the same inputs give the same bits.
+** from the unrounded delta.  The tensor cores cut sums off instead of rounding them (up to 7e-9 of a sum per term);
+** sums are therefore taken in runs that are added up rounded: 512 terms of a logit of the loss, 256 of fp32
+** gradients, 16,384 of bf16 gradients and 4096 of the logits behind these.  Sums run in a fixed order: the
+** same inputs give the same bits.
 **
 ** Waits inside the kernels are bounded: a block that gives up (two seconds without progress) fills what it
 ** has not computed with NaN, which shows in nll, dx, dw and dbias.
