@@ -1646,7 +1646,7 @@ extern "C" int anni_head_workspace(const anni_head_call *c, int grad, size_t *by
 
 	if (rc != ANNI_OK || !bytes)
 		return rc != ANNI_OK ? rc : ANNI_E_ARG;
-	*bytes = plan_of(c, grad).bytes;
+	*bytes = workspace_of(c, grad);
 	return ANNI_OK;
 }
 

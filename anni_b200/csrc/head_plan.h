@@ -167,7 +167,8 @@ int split_dx(int64_t tokens, int64_t d, int64_t width, int terms, bool dw, int l
 	return best;
 }
 
-head_plan plan_of(const anni_head_call *c, int grad)
+/* `least`: stages of an epilogue of dw */
+head_plan plan_of(const anni_head_call *c, int grad, int least)
 {
 	head_plan p;
 	const int64_t t = std::max<int64_t>(c->tokens, 1);
@@ -192,12 +193,27 @@ head_plan plan_of(const anni_head_call *c, int grad)
 	p.row = take(&p.bytes, t * 4);
 	p.delta = take(&p.bytes, (int64_t)p.piece * t * 2 * p.terms);
 	p.ldd = (int)up(c->d_model, 8);
-	p.splits = c->dx ? split_dx(t, c->d_model, std::min(p.piece, c->vocab), p.terms, c->dw != NULL,
-	    epilogue_of_dw(c->dw, c->lddw, c->grad_dtype == ANNI_DT_BF16, (c->flags & ANNI_HEAD_ACCUMULATE) != 0)) : 1;
+	p.splits = c->dx ? split_dx(t, c->d_model, std::min(p.piece, c->vocab), p.terms, c->dw != NULL, least) : 1;
 	p.parts = c->dx && (p.splits > 1 || p.piece < c->vocab);
 	p.dxp = take(&p.bytes, p.parts ? p.splits * t * p.ldd * 4 : 0);
 	p.dbp = take(&p.bytes, c->dbias ? up(t, HEAD_HALF) / HEAD_HALF * c->vocab * 4 : 0);
 	return p;
+}
+
+head_plan plan_of(const anni_head_call *c, int grad)
+{
+	return plan_of(c, grad, epilogue_of_dw(c->dw, c->lddw, c->grad_dtype == ANNI_DT_BF16,
+	    (c->flags & ANNI_HEAD_ACCUMULATE) != 0));
+}
+
+/* bytes of workspace wherever dw lies, and whether it is added to or not: the parts of dx depend on it */
+size_t workspace_of(const anni_head_call *c, int grad)
+{
+	size_t most = 0;
+
+	for (int least : { HEAD_EPI_STAGES, HEAD_EPI_STAGES_ADD, HEAD_EPI_STAGES_ODD })
+		most = std::max(most, plan_of(c, grad, least).bytes);
+	return most;
 }
 
 }	/* namespace */
