@@ -83,6 +83,8 @@ class MultiStep:
         params = list(params)
         if not params:
             raise ValueError("MultiStep: the list of tensors is empty")
+        if state_dtype == DT_Q8 and moments is not None and scales is None:
+            raise ValueError("MultiStep: 8-bit moments come with their scales")
         n = len(params)
         grads = [None] * n if grads is None else list(grads)
         if grad_dtype is None:
