@@ -188,7 +188,7 @@ class MultiStep:
     def moments(self):
         """m and v as lists of fp32 tensors of the parameters' shapes (copies in the 8-bit form)."""
         if self.state_dtype == DT_F32:
-            return self.m, self.v
+            return tuple([x.view(p.shape) for x, p in zip(xs, self.params)] for xs in (self.m, self.v))
         return ([decode(x, s).view(p.shape) for x, s, p in zip(self.m, self.m_scale, self.params)],
                 [decode(x, s).view(p.shape) for x, s, p in zip(self.v, self.v_scale, self.params)])
 
