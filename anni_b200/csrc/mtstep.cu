@@ -912,15 +912,6 @@ static int check_tensor(const anni_mt_tensor *t, int state_dtype, std::vector<ra
 	return ANNI_OK;
 }
 
-/*
-** What the host has written to the device on the legacy stream is there when this returns.  cudaMemset and cudaMemcpy
-** from pageable memory may return before; a step on a non-blocking stream does not wait for them.
-*/
-static bool landed(void)
-{
-	return cudaStreamSynchronize(cudaStreamLegacy) == cudaSuccess;
-}
-
 static int create(const anni_mt_tensor *list, int n, anni_mtstep *h)
 {
 	std::vector<mt_desc> desc((size_t)n);
@@ -974,7 +965,7 @@ static int create(const anni_mt_tensor *list, int n, anni_mtstep *h)
 	    || cudaMemcpy(h->desc, desc.data(), (size_t)n * sizeof(mt_desc), cudaMemcpyHostToDevice) != cudaSuccess
 	    || cudaMemcpy(h->grad, grads.data(), (size_t)n * sizeof(void *), cudaMemcpyHostToDevice) != cudaSuccess
 	    || cudaMemcpy(h->tile_of, table.data(), table.size() * sizeof(uint32_t), cudaMemcpyHostToDevice) != cudaSuccess
-	    || !landed()) {
+	    || !anni_landed()) {
 		(void)cudaGetLastError();
 		return ANNI_E_CUDA;
 	}
@@ -1119,7 +1110,7 @@ extern "C" int anni_mtstep_status_read(anni_mtstep *h, anni_optstep_status *out,
 		head.error = 0;
 		head.bar_count = 0;
 		head.done_ticket = 0;
-		if (cudaMemcpy(h->ctl, &head, nb, cudaMemcpyHostToDevice) != cudaSuccess || !landed())
+		if (cudaMemcpy(h->ctl, &head, nb, cudaMemcpyHostToDevice) != cudaSuccess || !anni_landed())
 			return ANNI_E_CUDA;
 	}
 	return ANNI_OK;

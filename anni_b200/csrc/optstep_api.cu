@@ -234,7 +234,7 @@ extern "C" int anni_optstep_create(const anni_optstep_config *cfg, anni_optstep 
 	    || cudaMemcpy(h->d_seg_off, off, (size_t)(h->n_seg + 1) * sizeof(int64_t),
 	    cudaMemcpyHostToDevice) != cudaSuccess
 	    || cudaMemcpy(h->d_seg_flags, flg, (size_t)h->n_seg * sizeof(uint32_t),
-	    cudaMemcpyHostToDevice) != cudaSuccess) {
+	    cudaMemcpyHostToDevice) != cudaSuccess || !anni_landed()) {
 		anni_optstep_destroy(h);
 		return ANNI_E_CUDA;
 	}
@@ -474,7 +474,7 @@ extern "C" int anni_optstep_set_derived(anni_optstep *h, const anni_seg_derived 
 	    || cudaMemcpy(h->d_aux, aux, (size_t)h->n_seg * sizeof(anni_seg_derived),
 	    cudaMemcpyHostToDevice) != cudaSuccess
 	    || cudaMemcpy(h->d_tile_prefix, prefix, (size_t)(h->n_seg + 1) * sizeof(int64_t),
-	    cudaMemcpyHostToDevice) != cudaSuccess) {
+	    cudaMemcpyHostToDevice) != cudaSuccess || !anni_landed()) {
 		free(prefix);
 		return ANNI_E_CUDA;
 	}
@@ -776,7 +776,7 @@ extern "C" int anni_optstep_status_read(anni_optstep *h, anni_optstep_status *ou
 		head.bar_count = 0;
 		head.norm_ticket = 0;
 		head.done_ticket = 0;
-		if (cudaMemcpy(h->ctl, &head, nb, cudaMemcpyHostToDevice) != cudaSuccess)
+		if (cudaMemcpy(h->ctl, &head, nb, cudaMemcpyHostToDevice) != cudaSuccess || !anni_landed())
 			return ANNI_E_CUDA;
 	}
 	return ANNI_OK;
@@ -800,7 +800,7 @@ extern "C" int anni_optstep_loss_scale_init(anni_optstep *h, double scale, int g
 	head.ls_min = min_scale;
 	head.ls_max = max_scale;
 	head.good_steps = 0;
-	return cudaMemcpy(h->ctl, &head, nb, cudaMemcpyHostToDevice) == cudaSuccess
+	return cudaMemcpy(h->ctl, &head, nb, cudaMemcpyHostToDevice) == cudaSuccess && anni_landed()
 	    ? ANNI_OK : ANNI_E_CUDA;
 }
 

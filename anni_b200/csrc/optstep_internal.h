@@ -190,6 +190,15 @@ void	anni_op_end(int slot, void *stream);
 int	anni_colsum_register(const float *host, float *dev, int cols);
 void	anni_colsum_forget(const void *dev_lo, const void *dev_hi);
 
+/*
+** What the host has written to the device on the legacy stream is there when this returns.  cudaMemset and cudaMemcpy
+** from pageable memory may return before; a step on a non-blocking stream does not wait for them.
+*/
+static inline bool anni_landed(void)
+{
+	return cudaStreamSynchronize(cudaStreamLegacy) == cudaSuccess;
+}
+
 #ifdef __cplusplus
 }
 #endif
