@@ -9,8 +9,8 @@
 **   grad    dx = delta W^T of the piece, added to an fp32 sum over the pieces, and dw = x^T delta of the piece, stored
 **           or added to the gradient; together, so that the tiles of one fill the rounds that the other leaves open
 ** Bound by the tensor cores: 2 T D V operations each (the logits twice, since they are not kept).  4096 rows of 1536
-** against 100,000 entries: loss 867 us (1.45 PFLOP/s, 0.86 of the rate of a library product), delta 966, dx and dw 1.7 ms
-** one by one; back to back at the power limit 4.2 ms in all, where four library products would take 3.6 ms.
+** against 100,000 entries: loss 838 us (1.50 PFLOP/s, 0.89 of the rate of a library product), delta 902, dx and dw 1.7 ms
+** one by one; back to back at the power limit 4.1 ms in all, where four library products would take 3.6 ms.
 **
 ** Two blocks (a cluster on two neighbouring SMs) work on a 256 x 256 tile: each keeps 128 rows of the result
 ** and loads its 128 rows of the one operand and 128 of the other by TMA into a ring of HEAD_STAGES stages; one
@@ -536,6 +536,12 @@ __device__ __forceinline__ void loss_epilogue(const gemm_args &g, const tile_at 
 	}
 }
 
+/*
+** Softmax minus one-hot, times the row's factor.  As an operand of a bf16 product it has to be bf16: for bf16 gradients
+** one term, whose rounding is as large as that of the result and adds to it as an independent one (off from 64 bits by
+** 1.9e-3 of the norm at 8192 x 1024 x 16,384, where the rounding of the result alone makes 1.7e-3; a second term would
+** take six products instead of four); for fp32 gradients three terms, which hold all 24 bits.
+*/
 __device__ __forceinline__ void delta_epilogue(const gemm_args &g, const tile_at &at, float (&acc)[4][32], const float *bias,
 	float (*sums)[HEAD_TN])
 {

@@ -344,7 +344,7 @@ class OptStep:
         """Loss of the head whose weights this engine steps: rows of nll for x (tokens, d_model) bf16 against
         ``target`` (tokens) int32, W read from the tensor ``w``'s twin, the bias (``b`` or None) from the master;
         with ``grad`` the gradients of ``grad_scale * sum(weight * nll)`` are added to the engine's gradients and,
-        if ``dx`` is given, written there (see anni_b200.head)."""
+        if ``dx`` is given, written there; nll itself carries no autograd history (see anni_b200.head)."""
         from .head import head_loss, head_loss_grad
         if self.segments is None or self.shard_off != 0 or self.shard_n != self.n_arena:
             raise ValueError("head_loss: needs an engine over a whole arena with named tensors")

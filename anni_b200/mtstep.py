@@ -72,7 +72,7 @@ class MultiStep:
     float8_e4m3fn, ``v`` float8_e5m2, ``m_scale`` and ``v_scale`` fp32 per 256 elements); zeroed state is
     made here unless ``moments=(m, v)`` and, for DT_Q8, ``scales=(m_scale, v_scale)`` hand it in.
 
-    Calls on one object belong on one stream.  Every call works on the list's device.  Gradients given to a call with
+    Calls on one object, this one among them, belong on one stream.  Every call works on the list's device.  Gradients given to a call with
     ``stream=`` stay allocated until that stream has finished with them, also when others have replaced them; those
     that a captured step reads are the caller's to keep for as long as it is replayed.
     """

@@ -52,7 +52,8 @@ extern "C" {
 ** One call.  ld*: elements from one row to the next, at least the row's length.  Any address and stride
 ** that the element type allows is taken; x and w on 16-byte addresses with strides that are multiples of
 ** 8 elements are read in place, others are copied into the workspace first (w: 4 bytes of traffic per
-** element).
+** element); anni_head_loss_grad copies x in any case, with zeros for the rows that have no gradient.
+** The loss of one or two rows copies nothing.  Outputs overlap neither each other nor what is read.
 */
 typedef struct anni_head_call {
 	const void	*x;		/* bf16 [tokens][ldx] */
@@ -82,7 +83,8 @@ typedef struct anni_head_call {
 
 /*
 ** Bytes of workspace that anni_head_loss (grad = 0) or anni_head_loss_grad (grad = 1) of this call need.
-** Only sizes, types, addresses of x and w, and which outputs are wanted are looked at.
+** Only sizes, types, addresses and strides of x and w, and which outputs are wanted are looked at: where dw and
+** dbias lie, and whether they are added to, makes no difference.
 */
 int	anni_head_workspace(const anni_head_call *c, int grad, size_t *bytes);
 /*
