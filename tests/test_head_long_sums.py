@@ -3,8 +3,21 @@ import pytest
 import torch
 
 from anni_b200.head import head_loss, head_loss_grad
+from test_head import BF, Exact, both, check_grads, check_loss, inputs
 
 gpu = pytest.mark.gpu
+
+
+@gpu
+@pytest.mark.parametrize("t,d,v", [(130, 4096, 520), (130, 4097, 520), (70, 9001, 300), (300, 64, 40000), (2050, 1000, 33000),
+                                   (16384, 64, 300), (16385, 64, 300), (40000, 72, 264)])
+def test_a_run_and_one_term_more(t, d, v):
+    """Each of the three sums at the length of one run, just beyond it, and of several."""
+    x, w, target, b = inputs(t, d, v, seed=41)
+    nll, lse, dx, dw, db = both(x, w, target, b, BF)
+    ex = Exact(x, w, target, b)
+    check_loss(ex, nll, lse)
+    check_grads(ex, BF, dx=dx, dw=dw, db=db)
 
 
 @gpu
